@@ -387,6 +387,155 @@ int fakla_decode_noalloc(const void* q, const void* k, const void* v,
                          int dtype, void* stream);
 
 /*
+ * fakla_gated_scan -- gated linear recurrence, per batch row and channel
+ *
+ *   a_t = sigmoid(gate_t) (FAKLA_ACT_SIGMOID) or gate_t (FAKLA_ACT_IDENTITY)
+ *   h_t = a_t h_{t-1} + (1 - a_t) x_t   (mix != 0)   or   a_t h_{t-1} + x_t
+ *
+ * Reference: none; the recurrent layer that stands beside FA-KLA, whose state
+ * is a vector per sequence instead of a matrix per head.
+ *
+ *   x, gate   : (B, T, D), unit stride over D; the batch and time strides are
+ *               given in elements (0 repeats a row), so both may be column
+ *               blocks of one projection's output
+ *   out       : (B, T, D) dense, written: h_t rounded to dtype
+ *   state_in  : (B, D) fp32, h before the first token, or NULL for zero
+ *   state_out : (B, D) fp32, written with h after the last token, or NULL;
+ *               may be state_in
+ *   saved     : fakla_gated_scan_saved_bytes() that the backward reads, or NULL
+ * h is carried in fp32. A gate of -inf (sigmoid) or 0 (identity) starts a new
+ * sequence at its token. Identity gates are decay factors: products of 128
+ * consecutive ones have to fit fp32.
+ */
+int fakla_gated_scan(const void* x, const void* gate, void* out, const float* state_in,
+                     float* state_out, void* saved, int64_t B, int64_t T, int64_t D,
+                     int64_t x_batch_stride, int64_t x_time_stride, int64_t gate_batch_stride,
+                     int64_t gate_time_stride, int act, int mix, int dtype, void* stream);
+
+size_t fakla_gated_scan_saved_bytes(int64_t B, int64_t T, int64_t D);
+
+/*
+ * fakla_gated_scan_backward -- gradients of fakla_gated_scan. With G_t =
+ * dout_t + a_{t+1} G_{t+1} (dstate_out added at the last token):
+ *   dx_t = G_t (1 - a_t) or G_t,  da_t = G_t (h_{t-1} - x_t) or G_t h_{t-1},
+ *   dgate_t = da_t a_t (1 - a_t) or da_t,  dstate_in = a_1 G_1.
+ *
+ * Reference: none.
+ *   x, gate, strides, act, mix : as given to the forward; saved : written by it
+ *   dout : (B, T, D) dense   dstate_out : (B, D) fp32 or NULL for zero
+ *   dx, dgate : (B, T, D) dense, written   dstate_in : (B, D) fp32, written, or NULL
+ */
+int fakla_gated_scan_backward(const void* x, const void* gate, const void* saved, const void* dout,
+                              const float* dstate_out, void* dx, void* dgate, float* dstate_in,
+                              int64_t B, int64_t T, int64_t D, int64_t x_batch_stride,
+                              int64_t x_time_stride, int64_t gate_batch_stride,
+                              int64_t gate_time_stride, int act, int mix, int dtype, void* stream);
+
+/*
+ * fakla_gated_scan_step -- one token of fakla_gated_scan for N sequences.
+ *   x, gate : (N, D), unit stride over D, row strides in elements
+ *   state_in, state_out : (N, D) fp32; state_out may be state_in (updated in
+ *   place), and otherwise does not overlap it     out : (N, D) dense, written
+ */
+int fakla_gated_scan_step(const void* x, const void* gate, void* out, const float* state_in,
+                          float* state_out, int64_t N, int64_t D, int64_t x_stride,
+                          int64_t gate_stride, int act, int mix, int dtype, void* stream);
+
+/*
+ * fakla_token_logprobs -- per row of logits, with y = logits / temperature and
+ * lse = log sum_j e^{y_j}:
+ *
+ *   logprobs     = y_target - lse                (0 where target == ignore_index)
+ *   entropy      = -sum_j p_j log p_j,  p_j = e^{y_j - lse}
+ *   top_ids      = the top_k largest logits, descending, the lower index first
+ *                  among equals;  top_logprobs = their y - lse
+ *
+ * Reference: none; scores the vocabulary head's output.
+ *
+ *   logits  : row (i, r) of batch x rows starts at i * batch_stride +
+ *             r * row_stride elements and holds vocab values
+ *   targets : (batch, rows)      logprobs, entropy : (batch, rows) fp32, written
+ *   top_logprobs, top_ids : (batch, rows, top_k), written; NULL with top_k = 0
+ *   stats   : (batch, rows, 2) fp32 that the backward reads, or NULL
+ * top_k <= 32 and <= vocab; vocab <= 2^20. A row of nothing but -inf has
+ * log probabilities -inf and entropy 0; a row with a NaN or +inf gives NaN and
+ * top_ids -1. A target outside [0, vocab) other than ignore_index gives NaN
+ * and sets the device status (FAKLA_ERR_INVALID_ARG).
+ */
+int fakla_token_logprobs(const void* logits, const int64_t* targets, float* logprobs,
+                         float* entropy, float* top_logprobs, int64_t* top_ids, float* stats,
+                         int64_t batch, int64_t rows, int64_t vocab, int64_t batch_stride,
+                         int64_t row_stride, int top_k, float temperature, int64_t ignore_index,
+                         int dtype, void* stream);
+
+/*
+ * fakla_token_logprobs_backward -- the gradient of the above into the logits:
+ *   dlogits_j = (w (1[j = target] - p_j) - dentropy p_j (log p_j + entropy)
+ *                + sum_k dtop_k (1[j = top_ids_k] - p_j)) / temperature
+ * with w = dlogprobs, 0 where the target is ignored. A row of nothing but
+ * -inf gets 0; one with a NaN, a +inf or a bad target gets NaN.
+ *
+ * Reference: none.
+ *   targets, entropy, top_ids, stats : as given to and written by the forward
+ *   dlogprobs, dentropy : (batch, rows) or NULL for zero
+ *   dtop_logprobs : (batch, rows, top_k) or NULL for zero
+ *   dlogits : (batch, rows, vocab) dense, written; logits' dtype
+ */
+int fakla_token_logprobs_backward(const void* logits, const int64_t* targets, const float* stats,
+                                  const float* entropy, const int64_t* top_ids,
+                                  const float* dlogprobs, const float* dentropy,
+                                  const float* dtop_logprobs, void* dlogits, int64_t batch,
+                                  int64_t rows, int64_t vocab, int64_t batch_stride,
+                                  int64_t row_stride, int top_k, float temperature,
+                                  int64_t ignore_index, int dtype, void* stream);
+
+/*
+ * fakla_distill_topk -- per row, the KL divergence of the model's distribution
+ * p = softmax(logits / temperature) from a teacher's q, known by its largest
+ * logits t_k at the vocabulary entries i_k:
+ *
+ *   teacher_lse NULL : q = softmax_k(t_k / temperature)
+ *                      loss = sum_k q_k (log q_k - log p_{i_k})
+ *   otherwise        : q_k = e^{t_k / temperature - teacher_lse}, where
+ *                      teacher_lse is log sum_j e^{t_j / temperature} over the
+ *                      teacher's whole vocabulary, and what is left over,
+ *                      q_r = max(0, 1 - sum_k q_k), is set against the model's
+ *                      mass outside of the i_k:  loss += q_r (log q_r - log p_r)
+ *
+ * Reference: none; trains the model of the vocabulary head's output.
+ *
+ *   logits : as in fakla_token_logprobs
+ *   teacher_ids, teacher_logits : (batch, rows, entries); an id of -1 is no entry
+ *   teacher_lse : (batch, rows) or NULL      loss : (batch, rows) fp32, written
+ *   stats : (batch, rows, 8) fp32 that the backward reads, or NULL
+ * entries <= 256, vocab <= 2^20. A row without an entry (or, without
+ * teacher_lse, with none above -inf) gives 0. Entries of the same id count
+ * each. An id below -1 or >= vocab gives NaN and sets the device status
+ * (FAKLA_ERR_INVALID_ARG).
+ */
+int fakla_distill_topk(const void* logits, const int64_t* teacher_ids, const float* teacher_logits,
+                       const float* teacher_lse, float* loss, float* stats, int64_t batch,
+                       int64_t rows, int64_t vocab, int64_t batch_stride, int64_t row_stride,
+                       int entries, float temperature, int dtype, void* stream);
+
+/*
+ * fakla_distill_topk_backward -- the gradient of the above into the logits,
+ * with Q = sum_k q_k and S the set of the i_k:
+ *   dlogits_j = dloss / temperature * (p_j (Q + q_r) - sum_{k: i_k = j} q_k
+ *               - 1[j not in S] q_r p_j / p_r)
+ *
+ * Reference: none.
+ *   stats : written by the forward     dloss : (batch, rows)
+ *   dlogits : (batch, rows, vocab) dense, written; logits' dtype
+ */
+int fakla_distill_topk_backward(const void* logits, const int64_t* teacher_ids,
+                                const float* teacher_logits, const float* teacher_lse,
+                                const float* stats, const float* dloss, void* dlogits,
+                                int64_t batch, int64_t rows, int64_t vocab, int64_t batch_stride,
+                                int64_t row_stride, int entries, float temperature, int dtype,
+                                void* stream);
+
+/*
  * fakla_device_status -- synchronise `stream` and return (then clear) the
  * device-side status word that kernels set when a bounded wait expires
  * (FAKLA_ERR_TIMEOUT) or a device-side check fails. FAKLA_OK if clean.

@@ -71,6 +71,14 @@ SIGNATURES = {
     "fakla_decode": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _p, _sz, _p]),
     "fakla_decode_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64, _int]),
     "fakla_decode_noalloc": (_int, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _int, _p]),
+    "fakla_gated_scan": (_int, [_p] * 6 + [_i64] * 7 + [_int, _int, _int, _p]),
+    "fakla_gated_scan_saved_bytes": (_sz, [_i64, _i64, _i64]),
+    "fakla_gated_scan_backward": (_int, [_p] * 8 + [_i64] * 7 + [_int, _int, _int, _p]),
+    "fakla_gated_scan_step": (_int, [_p] * 5 + [_i64] * 4 + [_int, _int, _int, _p]),
+    "fakla_token_logprobs": (_int, [_p] * 7 + [_i64] * 5 + [_int, ctypes.c_float, _i64, _int, _p]),
+    "fakla_token_logprobs_backward": (_int, [_p] * 9 + [_i64] * 5 + [_int, ctypes.c_float, _i64, _int, _p]),
+    "fakla_distill_topk": (_int, [_p] * 6 + [_i64] * 5 + [_int, ctypes.c_float, _int, _p]),
+    "fakla_distill_topk_backward": (_int, [_p] * 7 + [_i64] * 5 + [_int, ctypes.c_float, _int, _p]),
     "fakla_device_status": (_int, [_p]),
 }
 

@@ -6,3 +6,5 @@ from .interface import (  # noqa: F401
     fa_kla_prefill,
     phi_map,
 )
+from .logits import TokenLogprobs, distill_topk, token_logprobs  # noqa: F401
+from .recurrence import gated_scan, gated_scan_step  # noqa: F401

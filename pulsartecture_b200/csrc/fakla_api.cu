@@ -724,3 +724,280 @@ extern "C" int fakla_decode(const void* q, const void* k, const void* v, const v
   if (e != cudaSuccess) return cuda_fail(e, "decode launch");
   return FAKLA_OK;
 }
+
+// ---------------------------------------------------------------------------
+// Gated linear recurrence
+// ---------------------------------------------------------------------------
+namespace {
+// Sizes and form shared by the three gated-scan entry points. One block takes
+// at least one (batch row, 32 channels) pair, so their number fits a grid.
+int check_gated_scan(int64_t B, int64_t T, int64_t D, int act, int dtype) {
+  int rc = check_dtype(dtype);
+  if (rc) return rc;
+  if (B < 1 || T < 1 || D < 1)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "sizes must be positive (B=%lld T=%lld D=%lld)", (long long)B,
+                           (long long)T, (long long)D);
+  if (act != FAKLA_ACT_SIGMOID && act != FAKLA_ACT_IDENTITY)
+    return fakla_set_error(FAKLA_ERR_UNSUPPORTED, "gate activation %d is not sigmoid or identity", act);
+  if (D > INT32_MAX || B > INT32_MAX || B * ((D + 31) / 32) > INT32_MAX / 16)
+    return fakla_set_error(FAKLA_ERR_UNSUPPORTED, "B=%lld x D=%lld channels exceed one launch", (long long)B,
+                           (long long)D);
+  return FAKLA_OK;
+}
+}  // namespace
+
+extern "C" size_t fakla_gated_scan_saved_bytes(int64_t B, int64_t T, int64_t D) {
+  if (B < 1 || T < 1 || D < 1) return 0;
+  return fakla::gated_scan_saved_bytes(B, T, D);
+}
+
+extern "C" int fakla_gated_scan(const void* x, const void* gate, void* out, const float* state_in, float* state_out,
+                                void* saved, int64_t B, int64_t T, int64_t D, int64_t x_batch_stride,
+                                int64_t x_time_stride, int64_t gate_batch_stride, int64_t gate_time_stride, int act,
+                                int mix, int dtype, void* stream) {
+  int rc = check_gated_scan(B, T, D, act, dtype);
+  if (rc) return rc;
+  if (!x || !gate || !out) return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate and out must be non-NULL");
+  DeviceInfo* d = nullptr;
+  if ((rc = require_device(&d))) return rc;
+  fakla::GatedScanArgs p = {};
+  p.x = x;
+  p.gate = gate;
+  p.x_batch = x_batch_stride;
+  p.x_time = x_time_stride;
+  p.gate_batch = gate_batch_stride;
+  p.gate_time = gate_time_stride;
+  p.B = B;
+  p.T = T;
+  p.D = D;
+  p.act = act;
+  p.mix = mix != 0;
+  p.state_in = state_in;
+  p.state_out = state_out;
+  p.out = out;
+  p.saved = (float*)saved;
+  cudaError_t e = fakla::launch_gated_scan(dtype, p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "gated scan launch");
+  return FAKLA_OK;
+}
+
+extern "C" int fakla_gated_scan_backward(const void* x, const void* gate, const void* saved, const void* dout,
+                                         const float* dstate_out, void* dx, void* dgate, float* dstate_in, int64_t B,
+                                         int64_t T, int64_t D, int64_t x_batch_stride, int64_t x_time_stride,
+                                         int64_t gate_batch_stride, int64_t gate_time_stride, int act, int mix,
+                                         int dtype, void* stream) {
+  int rc = check_gated_scan(B, T, D, act, dtype);
+  if (rc) return rc;
+  if (!x || !gate || !saved || !dout || !dx || !dgate)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate, saved, dout, dx and dgate must be non-NULL");
+  DeviceInfo* d = nullptr;
+  if ((rc = require_device(&d))) return rc;
+  fakla::GatedScanArgs p = {};
+  p.x = x;
+  p.gate = gate;
+  p.x_batch = x_batch_stride;
+  p.x_time = x_time_stride;
+  p.gate_batch = gate_batch_stride;
+  p.gate_time = gate_time_stride;
+  p.B = B;
+  p.T = T;
+  p.D = D;
+  p.act = act;
+  p.mix = mix != 0;
+  p.saved = (float*)const_cast<void*>(saved);
+  p.dout = dout;
+  p.dstate_out = dstate_out;
+  p.dx = dx;
+  p.dgate = dgate;
+  p.dstate_in = dstate_in;
+  cudaError_t e = fakla::launch_gated_scan_backward(dtype, p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "gated scan backward launch");
+  return FAKLA_OK;
+}
+
+extern "C" int fakla_gated_scan_step(const void* x, const void* gate, void* out, const float* state_in,
+                                     float* state_out, int64_t N, int64_t D, int64_t x_stride, int64_t gate_stride,
+                                     int act, int mix, int dtype, void* stream) {
+  int rc = check_gated_scan(N, 1, D, act, dtype);
+  if (rc) return rc;
+  if (!x || !gate || !out || !state_in || !state_out)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate, out, state_in and state_out must be non-NULL");
+  DeviceInfo* d = nullptr;
+  if ((rc = require_device(&d))) return rc;
+  fakla::GatedScanArgs p = {};
+  p.x = x;
+  p.gate = gate;
+  p.x_batch = x_stride;
+  p.gate_batch = gate_stride;
+  p.B = N;
+  p.T = 1;
+  p.D = D;
+  p.act = act;
+  p.mix = mix != 0;
+  p.state_in = state_in;
+  p.state_out = state_out;
+  p.out = out;
+  cudaError_t e = fakla::launch_gated_scan_step(dtype, p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "gated scan step launch");
+  return FAKLA_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Rows of logits
+// ---------------------------------------------------------------------------
+namespace {
+constexpr int64_t kMaxVocab = 1 << 20;
+constexpr int kMaxTopK = 32;
+constexpr int kMaxEntries = 256;
+
+int check_logits(const void* logits, int64_t batch, int64_t rows, int64_t vocab, float temperature, int dtype,
+                 fakla::LogitsArgs* p) {
+  int rc = check_dtype(dtype);
+  if (rc) return rc;
+  if (!logits) return fakla_set_error(FAKLA_ERR_INVALID_ARG, "logits must be non-NULL");
+  if (batch < 1 || rows < 1 || vocab < 1)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "sizes must be positive (batch=%lld rows=%lld vocab=%lld)",
+                           (long long)batch, (long long)rows, (long long)vocab);
+  if (vocab > kMaxVocab)
+    return fakla_set_error(FAKLA_ERR_UNSUPPORTED, "vocab %lld above %lld", (long long)vocab, (long long)kMaxVocab);
+  if (batch > INT32_MAX || rows > INT32_MAX || batch * rows > INT32_MAX / 16)
+    return fakla_set_error(FAKLA_ERR_UNSUPPORTED, "%lld x %lld rows exceed one launch", (long long)batch,
+                           (long long)rows);
+  // the reciprocal has to be a normal number too
+  if (!(temperature >= 1e-30f && temperature <= 1e30f))
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "temperature must be in [1e-30, 1e30], got %g", (double)temperature);
+  p->logits = logits;
+  p->batch = batch;
+  p->rows = rows;
+  p->vocab = vocab;
+  p->inv_temperature = 1.f / temperature;
+  return FAKLA_OK;
+}
+
+int check_top_k(int top_k, int64_t vocab) {
+  if (top_k < 0 || top_k > kMaxTopK || top_k > vocab)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "top_k %d is not in [0, min(%d, vocab)]", top_k, kMaxTopK);
+  return FAKLA_OK;
+}
+
+int check_entries(int entries) {
+  if (entries < 1 || entries > kMaxEntries)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "entries %d is not in [1, %d]", entries, kMaxEntries);
+  return FAKLA_OK;
+}
+}  // namespace
+
+extern "C" int fakla_token_logprobs(const void* logits, const int64_t* targets, float* logprobs, float* entropy,
+                                    float* top_logprobs, int64_t* top_ids, float* stats, int64_t batch, int64_t rows,
+                                    int64_t vocab, int64_t batch_stride, int64_t row_stride, int top_k,
+                                    float temperature, int64_t ignore_index, int dtype, void* stream) {
+  fakla::LogitsArgs p = {};
+  int rc = check_logits(logits, batch, rows, vocab, temperature, dtype, &p);
+  if (!rc) rc = check_top_k(top_k, vocab);
+  if (rc) return rc;
+  if (!targets || !logprobs || !entropy || (top_k > 0 && (!top_logprobs || !top_ids)))
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG,
+                           "targets, logprobs, entropy and (with top_k) top_logprobs, top_ids must be non-NULL");
+  DeviceInfo* d = nullptr;
+  if ((rc = require_device(&d))) return rc;
+  p.batch_stride = batch_stride;
+  p.row_stride = row_stride;
+  p.status = d->st();
+  p.targets = targets;
+  p.ignore_index = ignore_index;
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.top_logprobs = top_logprobs;
+  p.top_ids = top_ids;
+  p.top_k = top_k;
+  p.stats = stats;
+  cudaError_t e = fakla::launch_token_logprobs(dtype, p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "token logprobs launch");
+  return FAKLA_OK;
+}
+
+extern "C" int fakla_token_logprobs_backward(const void* logits, const int64_t* targets, const float* stats,
+                                             const float* entropy, const int64_t* top_ids, const float* dlogprobs,
+                                             const float* dentropy, const float* dtop_logprobs, void* dlogits,
+                                             int64_t batch, int64_t rows, int64_t vocab, int64_t batch_stride,
+                                             int64_t row_stride, int top_k, float temperature, int64_t ignore_index,
+                                             int dtype, void* stream) {
+  fakla::LogitsArgs p = {};
+  int rc = check_logits(logits, batch, rows, vocab, temperature, dtype, &p);
+  if (!rc) rc = check_top_k(top_k, vocab);
+  if (rc) return rc;
+  if (!targets || !stats || !entropy || !dlogits || (dtop_logprobs && (!top_ids || top_k == 0)))
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG,
+                           "targets, stats, entropy, dlogits and (with dtop_logprobs) top_ids must be non-NULL");
+  DeviceInfo* d = nullptr;
+  if ((rc = require_device(&d))) return rc;
+  p.batch_stride = batch_stride;
+  p.row_stride = row_stride;
+  p.targets = targets;
+  p.ignore_index = ignore_index;
+  p.stats = const_cast<float*>(stats);
+  p.entropy = const_cast<float*>(entropy);
+  p.top_ids = const_cast<int64_t*>(top_ids);
+  p.top_k = dtop_logprobs ? top_k : 0;
+  p.dlogprobs = dlogprobs;
+  p.dentropy = dentropy;
+  p.dtop_logprobs = dtop_logprobs;
+  p.dlogits = dlogits;
+  cudaError_t e = fakla::launch_token_logprobs_backward(dtype, p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "token logprobs backward launch");
+  return FAKLA_OK;
+}
+
+extern "C" int fakla_distill_topk(const void* logits, const int64_t* teacher_ids, const float* teacher_logits,
+                                  const float* teacher_lse, float* loss, float* stats, int64_t batch, int64_t rows,
+                                  int64_t vocab, int64_t batch_stride, int64_t row_stride, int entries,
+                                  float temperature, int dtype, void* stream) {
+  fakla::LogitsArgs p = {};
+  int rc = check_logits(logits, batch, rows, vocab, temperature, dtype, &p);
+  if (!rc) rc = check_entries(entries);
+  if (rc) return rc;
+  if (!teacher_ids || !teacher_logits || !loss)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "teacher_ids, teacher_logits and loss must be non-NULL");
+  DeviceInfo* d = nullptr;
+  if ((rc = require_device(&d))) return rc;
+  p.batch_stride = batch_stride;
+  p.row_stride = row_stride;
+  p.status = d->st();
+  p.teacher_ids = teacher_ids;
+  p.teacher_logits = teacher_logits;
+  p.teacher_lse = teacher_lse;
+  p.entries = entries;
+  p.loss = loss;
+  p.stats = stats;
+  cudaError_t e = fakla::launch_distill(dtype, p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "distill launch");
+  return FAKLA_OK;
+}
+
+extern "C" int fakla_distill_topk_backward(const void* logits, const int64_t* teacher_ids,
+                                           const float* teacher_logits, const float* teacher_lse, const float* stats,
+                                           const float* dloss, void* dlogits, int64_t batch, int64_t rows,
+                                           int64_t vocab, int64_t batch_stride, int64_t row_stride, int entries,
+                                           float temperature, int dtype, void* stream) {
+  fakla::LogitsArgs p = {};
+  int rc = check_logits(logits, batch, rows, vocab, temperature, dtype, &p);
+  if (!rc) rc = check_entries(entries);
+  if (rc) return rc;
+  if (!teacher_ids || !teacher_logits || !stats || !dloss || !dlogits)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG,
+                           "teacher_ids, teacher_logits, stats, dloss and dlogits must be non-NULL");
+  DeviceInfo* d = nullptr;
+  if ((rc = require_device(&d))) return rc;
+  p.batch_stride = batch_stride;
+  p.row_stride = row_stride;
+  p.teacher_ids = teacher_ids;
+  p.teacher_logits = teacher_logits;
+  p.teacher_lse = teacher_lse;
+  p.entries = entries;
+  p.stats = const_cast<float*>(stats);
+  p.dloss = dloss;
+  p.dlogits = dlogits;
+  cudaError_t e = fakla::launch_distill_backward(dtype, p, (cudaStream_t)stream);
+  if (e != cudaSuccess) return cuda_fail(e, "distill backward launch");
+  return FAKLA_OK;
+}

@@ -139,4 +139,57 @@ cudaError_t launch_qkv_sm100(const void* x, const void* W, const void* bias, con
                              void* out, int64_t rows, int64_t K, int64_t feat, int64_t vdim,
                              int64_t heads, cudaStream_t stream, int* status, bool* encoded);
 
+// Gated linear recurrence (simt_gated_scan.cu). Strides are in elements; out,
+// dout, dx and dgate are dense (B, T, D).
+struct GatedScanArgs {
+  const void *x, *gate;
+  int64_t x_batch, x_time, gate_batch, gate_time;
+  int64_t B, T, D;
+  int act;   // FAKLA_ACT_SIGMOID or FAKLA_ACT_IDENTITY
+  bool mix;  // b = (1 - a) x, else x
+  const float* state_in;  // (B, D) or null for zero
+  float* state_out;       // (B, D) or null
+  void* out;
+  float* saved;  // forward: written unless null; backward: read
+  const void* dout;
+  const float* dstate_out;  // (B, D) or null for zero
+  void *dx, *dgate;
+  float* dstate_in;  // (B, D) or null
+};
+size_t gated_scan_saved_bytes(int64_t B, int64_t T, int64_t D);
+cudaError_t launch_gated_scan(int dtype, const GatedScanArgs& p, cudaStream_t stream);
+cudaError_t launch_gated_scan_backward(int dtype, const GatedScanArgs& p, cudaStream_t stream);
+cudaError_t launch_gated_scan_step(int dtype, const GatedScanArgs& p, cudaStream_t stream);
+
+// Rows of logits (simt_logits.cu): row (i, r) starts at logits +
+// i * batch_stride + r * row_stride elements; everything else is dense over
+// batch * rows.
+struct LogitsArgs {
+  const void* logits;
+  int64_t batch, rows, vocab, batch_stride, row_stride;
+  float inv_temperature;
+  float* stats;  // forward: written unless null; backward: read
+  int* status;
+  // token log probabilities
+  const int64_t* targets;
+  int64_t ignore_index;
+  float *logprobs, *entropy, *top_logprobs;
+  int64_t* top_ids;
+  int top_k;
+  // distillation
+  const int64_t* teacher_ids;
+  const float *teacher_logits, *teacher_lse;
+  int entries;
+  float* loss;
+  // gradients (null = zero)
+  const float *dlogprobs, *dentropy, *dtop_logprobs, *dloss;
+  void* dlogits;
+};
+constexpr int kTokenStats = 2;    // floats per row that the forward keeps for the backward
+constexpr int kDistillStats = 8;
+cudaError_t launch_token_logprobs(int dtype, const LogitsArgs& p, cudaStream_t stream);
+cudaError_t launch_token_logprobs_backward(int dtype, const LogitsArgs& p, cudaStream_t stream);
+cudaError_t launch_distill(int dtype, const LogitsArgs& p, cudaStream_t stream);
+cudaError_t launch_distill_backward(int dtype, const LogitsArgs& p, cudaStream_t stream);
+
 }  // namespace fakla

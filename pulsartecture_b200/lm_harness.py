@@ -10,6 +10,10 @@ measured:
     L x [ x += W_o TMLinKernelAttn(LN(x));  x += MoE(LN(x)) ]
     logits = head(LN(x))
 
+Layers named in ``recurrent_layers`` take GatedRecurrence in the place of
+TMLinKernelAttn. ``score``, ``loss`` and ``distill_loss`` go on from the logits
+with ``token_logprobs`` and ``distill_topk``.
+
 The MoE layer follows the reference's top-k gating (ultra_rwka/MoE/gating.py:
 112-145: the top-k gate logits, a softmax over those k, no noise at
 inference) over GELU MLP experts (the shape of ultra_rwka/MoE/branches.py
@@ -17,17 +21,21 @@ MLPBranch). The reference's IDAM memory and wavelet mixing are left out: the
 repository gives them no defaults, and the wavelet projection needs a
 backend operation the reference does not implement.
 
-Everything but the attention runs on PyTorch / cuBLAS; the attention
-sublayers are the FA-KLA kernels of this package.
+Everything but the token mixing and what follows the logits runs on PyTorch /
+cuBLAS; the attention sublayers are the FA-KLA kernels of this package, the
+recurrent ones its gated scan.
 """
 from __future__ import annotations
 
 import math
+from typing import Optional, Sequence
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .attention import TMLinKernelAttn
+from .attention import GatedRecurrence, TMLinKernelAttn
+from .backend.logits import TokenLogprobs, distill_topk, token_logprobs
 from .kernels import LearnablePositiveMap
 
 
@@ -81,17 +89,21 @@ class MoEFeedForward(nn.Module):
 
 
 class FaklaBlock(nn.Module):
-    """Pre-norm block: FA-KLA attention (with an output projection back to
-    d_model) and an MoE feed-forward, each added to the residual stream."""
+    """Pre-norm block: FA-KLA attention or a gated recurrence (with an output
+    projection back to d_model) and an MoE feed-forward, each added to the
+    residual stream."""
 
     def __init__(self, d_model: int, n_heads: int, head_dim: int, d_ff: int, n_experts: int, top_k: int,
-                 device=None, dtype=None):
+                 device=None, dtype=None, recurrent: bool = False):
         super().__init__()
         fk = {"device": device, "dtype": dtype}
         feat = n_heads * head_dim
         self.ln_attn = nn.LayerNorm(d_model, **fk)
-        self.attn = TMLinKernelAttn(d_model, LearnablePositiveMap(feat, feat, **fk), num_heads=n_heads,
-                                    qk_dim=head_dim, v_dim=head_dim, **fk)
+        if recurrent:
+            self.attn = GatedRecurrence(d_model, feat, **fk)
+        else:
+            self.attn = TMLinKernelAttn(d_model, LearnablePositiveMap(feat, feat, **fk), num_heads=n_heads,
+                                        qk_dim=head_dim, v_dim=head_dim, **fk)
         self.proj_out = nn.Linear(feat, d_model, **fk)
         self.ln_ff = nn.LayerNorm(d_model, **fk)
         self.ff = MoEFeedForward(d_model, d_ff, n_experts, top_k, **fk)
@@ -104,16 +116,20 @@ class FaklaBlock(nn.Module):
 class FaklaLM(nn.Module):
     """Token ids (B, T) -> next-token logits (B, T, vocab). Defaults: 12
     layers, d_model 1024, 16 FA-KLA heads of 64, top-2 of 8 experts with
-    d_ff 4096, vocabulary 32000."""
+    d_ff 4096, vocabulary 32000. ``recurrent_layers``: indices of the layers
+    that mix tokens by a gated recurrence instead of FA-KLA."""
 
     def __init__(self, vocab: int = 32000, d_model: int = 1024, n_layers: int = 12, n_heads: int = 16,
                  head_dim: int = 64, d_ff: int = 4096, n_experts: int = 8, top_k: int = 2, device=None,
-                 dtype=None):
+                 dtype=None, recurrent_layers: Sequence[int] = ()):
         super().__init__()
         fk = {"device": device, "dtype": dtype}
+        recurrent = set(recurrent_layers)
+        if not recurrent <= set(range(n_layers)):
+            raise ValueError(f"recurrent_layers {sorted(recurrent)} are not all in [0, {n_layers})")
         self.embed = nn.Embedding(vocab, d_model, **fk)
-        self.blocks = nn.ModuleList([FaklaBlock(d_model, n_heads, head_dim, d_ff, n_experts, top_k, **fk)
-                                     for _ in range(n_layers)])
+        self.blocks = nn.ModuleList([FaklaBlock(d_model, n_heads, head_dim, d_ff, n_experts, top_k, **fk,
+                                                recurrent=i in recurrent) for i in range(n_layers)])
         self.ln_f = nn.LayerNorm(d_model, **fk)
         self.head = nn.Linear(d_model, vocab, bias=False, **fk)
 
@@ -122,3 +138,27 @@ class FaklaLM(nn.Module):
         for blk in self.blocks:
             x = blk(x)
         return self.head(self.ln_f(x))
+
+    @torch.no_grad()
+    def score(self, ids: torch.Tensor, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+        """What the model gave the tokens ids[:, 1:] in their places: (B, T - 1)
+        log probabilities and entropies, with the top_k alternatives of each."""
+        return token_logprobs(self(ids)[:, :-1], ids[:, 1:], top_k=top_k, temperature=temperature)
+
+    def loss(self, ids: torch.Tensor, entropy_weight: float = 0.0, ignore_index: int = -100) -> torch.Tensor:
+        """Mean next-token cross entropy of ids (B, T), less entropy_weight times
+        the mean entropy over the same positions. Targets equal to ignore_index
+        (padding) are left out; such ids are embedded as token 0."""
+        targets = torch.cat([ids[:, 1:], torch.full_like(ids[:, :1], ignore_index)], dim=1)
+        counted = targets != ignore_index
+        r = token_logprobs(self(ids.masked_fill(ids == ignore_index, 0)), targets, ignore_index=ignore_index)
+        total = r.logprobs.sum()
+        if entropy_weight:
+            total = total + entropy_weight * r.entropy.masked_fill(~counted, 0.0).sum()
+        return -total / counted.sum().clamp_min(1)
+
+    def distill_loss(self, ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                     teacher_lse: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
+        """Mean over ids (B, T) of the KL divergence from a teacher's largest
+        logits, teacher_ids and teacher_logits (B, T, K)."""
+        return distill_topk(self(ids), teacher_ids, teacher_logits, teacher_lse, temperature=temperature).mean()
