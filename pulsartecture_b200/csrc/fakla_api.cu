@@ -761,6 +761,7 @@ extern "C" int fakla_gated_scan(const void* x, const void* gate, void* out, cons
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};
+  p.status = d->st();
   p.x = x;
   p.gate = gate;
   p.x_batch = x_batch_stride;
@@ -793,6 +794,7 @@ extern "C" int fakla_gated_scan_backward(const void* x, const void* gate, const 
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};
+  p.status = d->st();
   p.x = x;
   p.gate = gate;
   p.x_batch = x_batch_stride;
@@ -825,6 +827,7 @@ extern "C" int fakla_gated_scan_step(const void* x, const void* gate, void* out,
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};
+  p.status = d->st();
   p.x = x;
   p.gate = gate;
   p.x_batch = x_stride;

@@ -155,6 +155,7 @@ struct GatedScanArgs {
   const float* dstate_out;  // (B, D) or null for zero
   void *dx, *dgate;
   float* dstate_in;  // (B, D) or null
+  int* status;
 };
 size_t gated_scan_saved_bytes(int64_t B, int64_t T, int64_t D);
 cudaError_t launch_gated_scan(int dtype, const GatedScanArgs& p, cudaStream_t stream);
