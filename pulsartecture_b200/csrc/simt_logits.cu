@@ -2,145 +2,687 @@
 // largest entries, and the divergence from a teacher's largest logits, with
 // their gradients.
 //
-// With y = x / temperature, m = max y and s = sum_j e^{y_j - m}:
-//   log p_j = (y_j - m) - log s,  H = log s - (sum_j e^{y_j - m} (y_j - m)) / s,
-// both sums of one sign, so neither cancels. The backward recomputes p from m
-// and log s. Everything is fp32; dlogits are rounded once.
+// With c = log2(e) / temperature, m = max x, M = c m and y_j = c x_j - M (one
+// fused multiply-add, so y is exact but for its own rounding):
+//   s = sum_j 2^{y_j},  log p_j = ln 2 (y_j - log2 s),
+//   H = ln 2 (log2 s - (sum_j 2^{y_j} y_j) / s),
+// both parts of H of one sign, so they do not cancel. The forward reads a row
+// once: a thread keeps the maximum of what it has seen and rescales its sums
+// when that grows; threads, and the blocks of a cluster where a row is split,
+// merge theirs at the end in a fixed order. The backward recomputes p from m
+// and log2 s, reading the logits once more and storing nothing in between.
+// Memory bounds both: bf16 logits at 6.5 TB/s are 11 instructions per value on
+// 148 SMs, and the passes take 5 to 8. Everything is fp32; dlogits are rounded
+// once.
 //
-// A row of nothing but -inf (s = 0) keeps log s = +inf, which makes every p 0.
+// Rows whose maximum is past 10^6 / c (a temperature close to 0, masks of a
+// type's lowest value over all of a row) lose y in that form; they are summed
+// once more from (x - m) / temperature, by one block, scalar by scalar. A row
+// of nothing but -inf keeps log2 s = +inf, which makes every p 0.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
-#include <math_constants.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "fakla_common.cuh"
 #include "fakla_kernels.h"
+#include "sm100_umma.cuh"
 
 namespace fakla {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kUnroll = 4;      // 16-byte loads of a thread in flight
+constexpr int kMaxCluster = 8;  // the largest portable cluster
+constexpr int kMaxTop = 32;     // as fakla_token_logprobs takes; also the lanes of a warp
+constexpr int kMaxEntries = kThreads;
+constexpr int kCandidates = 1024;
+constexpr float kInf = __builtin_huge_valf();
+constexpr float kNaN = __builtin_nanf("");
+constexpr float kLog2e = 1.44269504f;
+constexpr float kLn2 = 0.693147181f;
+constexpr float kFar = 1e6f;         // |c x| up to which y is formed by one fma
+constexpr float kNear = 0.99f * kFar;  // and which a row's maximum keeps within
 
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ uint4 load_vec(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p));
+  return r;
+}
+
+// 16 bytes of logits as pairs of fp32.
 template <typename T>
-__device__ __forceinline__ const T* row_of(const LogitsArgs& p, int64_t row) {
-  return (const T*)p.logits + row / p.rows * p.batch_stride + row % p.rows * p.row_stride;
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int E = 4;
+  static __device__ __forceinline__ uint64_t pair(const uint4& v, int i) {
+    return i == 0 ? sm100::f2_make(v.x, v.y) : sm100::f2_make(v.z, v.w);
+  }
+  static __device__ __forceinline__ float max(const uint4& v) {
+    return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  // not below `low`; NaN stays
+  static __device__ __forceinline__ uint4 at_least(uint4 v, float low) {
+    auto f = [&](uint32_t x) {
+      float r;
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(x)), "f"(low));
+      return __float_as_uint(r);
+    };
+    return make_uint4(f(v.x), f(v.y), f(v.z), f(v.w));
+  }
+  static __device__ __forceinline__ uint4 put(const uint64_t* p) {
+    const float2 a = sm100::f2_split(p[0]), b = sm100::f2_split(p[1]);
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+  }
+};
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int E = 8;
+  static __device__ __forceinline__ uint32_t word(const uint4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+  }
+  static __device__ __forceinline__ __nv_bfloat162 two(uint32_t w) { return *reinterpret_cast<__nv_bfloat162*>(&w); }
+  static __device__ __forceinline__ uint32_t bits(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
+  static __device__ __forceinline__ uint64_t pair(const uint4& v, int i) { return sm100::f2_from_bf16x2(word(v, i)); }
+  static __device__ __forceinline__ float max(const uint4& v) {
+    const uint32_t w = bits(__hmax2(__hmax2(two(v.x), two(v.y)), __hmax2(two(v.z), two(v.w))));
+    return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ uint4 at_least(uint4 v, float low) {
+    const __nv_bfloat162 l = __bfloat162bfloat162(__float2bfloat16_rd(low));  // at or below it: y stays at or below 0
+    auto f = [&](uint32_t x) { return bits(__hmax2_nan(two(x), l)); };
+    return make_uint4(f(v.x), f(v.y), f(v.z), f(v.w));
+  }
+  static __device__ __forceinline__ uint4 put(const uint64_t* p) {
+    return make_uint4(sm100::pack_bf16x2(p[0]), sm100::pack_bf16x2(p[1]), sm100::pack_bf16x2(p[2]), sm100::pack_bf16x2(p[3]));
+  }
+};
+
+// A row in 16-byte vectors, with up to E - 1 single values before and after
+// them where the row does not start or end on 16 bytes.
+template <typename T>
+struct Row {
+  static constexpr int E = Vec<T>::E;
+  const T* x;
+  int V, lead, vectors, singles;
+  __device__ Row(const LogitsArgs& p, int64_t row) {
+    x = (const T*)p.logits + row / p.rows * p.batch_stride + row % p.rows * p.row_stride;
+    V = (int)p.vocab;
+    lead = (int)(-(intptr_t)x & 15) / (int)sizeof(T);
+    if (lead > V) lead = V;
+    vectors = (V - lead) / E;
+    singles = V - vectors * E;
+  }
+  __device__ const T* vec(int v) const { return x + lead + v * E; }
+  __device__ int single(int i) const { return i < lead ? i : i + vectors * E; }
+  // the place of value j: its vector, or -1 - (its number among the singles)
+  __device__ int place(int j) const {
+    if (j < lead) return -1 - j;
+    const int v = (j - lead) / E;
+    return v < vectors ? v : -1 - (j - vectors * E);
+  }
+};
+
+__device__ __forceinline__ float scale_of(const LogitsArgs& p) { return kLog2e * p.inv_temperature; }
+
+// What a row's values, or some of them, add up to.
+struct Sums {
+  float m;  // the largest value
+  float s;  // sum 2^y
+  float w;  // sum 2^y y
+  float t;  // sum 2^y outside of the teacher's entries
+};
+
+// M of a maximum m, kept finite for -inf.
+__device__ __forceinline__ float base_of(float m, float c) { return fmaxf(__fmul_rn(m, c), -kFar); }
+
+__device__ __forceinline__ void move_base(Sums& a, float from, float to) {
+  const float f = exp2_approx(from - to);
+  a.w = f * fmaf(from - to, a.s, a.w);
+  a.s *= f;
+  a.t *= f;
 }
 
-template <typename V, typename F>
-__device__ V block_reduce(V v, F f) {
-  __shared__ V part[32];
-  __syncthreads();
-  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
-  __syncthreads();
-  v = part[0];
-  for (int i = 1; i < blockDim.x / 32; ++i) v = f(v, part[i]);
-  return v;
+__device__ __forceinline__ Sums merge(Sums a, Sums b, float c) {
+  const float A = base_of(a.m, c), B = base_of(b.m, c);
+  if (A >= B) move_base(b, B, A);
+  else move_base(a, A, B);
+  return {fmaxf(a.m, b.m), a.s + b.s, a.w + b.w, a.t + b.t};
 }
-__device__ float block_sum(float v) { return block_reduce(v, [](float a, float b) { return a + b; }); }
-__device__ float block_max(float v) { return block_reduce(v, [](float a, float b) { return fmaxf(a, b); }); }
 
-// Order of the values (-0 as 0), then of the lower index.
+// One thread's running sums. WEIGHTED: the entropy's; REST: those outside of
+// the teacher's entries.
+template <typename T, bool WEIGHTED, bool REST>
+struct Running {
+  static constexpr int E = Vec<T>::E;
+  float m, M, c;
+  uint64_t c2, s2, w2, t2;
+  __device__ explicit Running(float c_) : m(-kInf), M(-kFar), c(c_), c2(sm100::f2_splat(c_)) {
+    s2 = w2 = t2 = sm100::f2_splat(0.f);
+  }
+  __device__ __forceinline__ void see(float most) {
+    if (most > m) {
+      m = most;
+      const float to = base_of(m, c);
+      const uint64_t f = sm100::f2_splat(exp2_approx(M - to));
+      if (WEIGHTED) w2 = sm100::f2_mul(f, sm100::f2_fma(sm100::f2_splat(M - to), s2, w2));
+      s2 = sm100::f2_mul(f, s2);
+      if (REST) t2 = sm100::f2_mul(f, t2);
+      M = to;
+    }
+  }
+  // member: bit i set where value i is one of the teacher's entries
+  __device__ __forceinline__ void add(uint4 v, uint32_t member) {
+    if (WEIGHTED) v = Vec<T>::at_least(v, -kFar / c);  // 2^y y is 0 there, not 0 times -inf
+    const uint64_t nM = sm100::f2_splat(-M);
+    uint64_t e[E / 2], all = 0;
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+      const uint64_t y = sm100::f2_fma(Vec<T>::pair(v, i), c2, nM);
+      const float2 f = sm100::f2_split(y);
+      e[i] = sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y)));
+      all = i == 0 ? e[i] : sm100::f2_add(all, e[i]);
+      if (WEIGHTED) w2 = sm100::f2_fma(e[i], y, w2);
+    }
+    s2 = sm100::f2_add(s2, all);
+    if (REST) {
+      if (member == 0) {
+        t2 = sm100::f2_add(t2, all);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) {
+          const float2 f = sm100::f2_split(e[i]);
+          t2 = sm100::f2_add(t2, sm100::f2_make(member >> (2 * i) & 1 ? 0u : __float_as_uint(f.x),
+                                                member >> (2 * i + 1) & 1 ? 0u : __float_as_uint(f.y)));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void add_single(float x, bool member) {
+    see(x);
+    const float y = fmaf(WEIGHTED ? (x < -kFar / c ? -kFar / c : x) : x, c, -M), e = exp2_approx(y);
+    s2 = sm100::f2_add(s2, sm100::f2_make(__float_as_uint(e), 0u));
+    if (WEIGHTED) w2 = sm100::f2_fma(sm100::f2_make(__float_as_uint(e), 0u), sm100::f2_make(__float_as_uint(y), 0u), w2);
+    if (REST && !member) t2 = sm100::f2_add(t2, sm100::f2_make(__float_as_uint(e), 0u));
+  }
+  __device__ Sums sums() const {
+    auto both = [](uint64_t v) { const float2 f = sm100::f2_split(v); return f.x + f.y; };
+    return {m, both(s2), WEIGHTED ? both(w2) : 0.f, REST ? both(t2) : 0.f};
+  }
+};
+
+// A number of vectors known when compiling.
+template <int N>
+struct Count {
+  __device__ constexpr operator int() const { return N; }
+};
+
+// Runs f(vectors, the first one's number, how many) on every thread's vectors
+// of [v0, v1), kUnroll at a time, kThreads apart.
+template <typename T, typename F>
+__device__ __forceinline__ void each_vectors(const Row<T>& row, int v0, int v1, F f) {
+  for (int v = v0 + threadIdx.x; v < v1; v += kUnroll * kThreads) {
+    uint4 raw[kUnroll];
+    const int n = (v1 - v + kThreads - 1) / kThreads;
+    if (n >= kUnroll) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) raw[u] = load_vec(row.vec(v + u * kThreads));
+      f(raw, v, Count<kUnroll>{});
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnroll - 1; ++u)
+        if (u < n) raw[u] = load_vec(row.vec(v + u * kThreads));
+      f(raw, v, n);
+    }
+  }
+}
+
+__device__ Sums block_merge(Sums a, float c) {
+  __shared__ Sums part[kWarps];
+  auto from = [&](int o) {
+    return Sums{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.w, o),
+                __shfl_xor_sync(~0u, a.t, o)};
+  };
+  for (int o = 16; o > 0; o >>= 1) {
+    const Sums b = from(o);
+    a = threadIdx.x & o ? merge(b, a, c) : merge(a, b, c);
+  }
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = a;
+  __syncthreads();
+  a = part[0];
+  for (int i = 1; i < kWarps; ++i) a = merge(a, part[i], c);
+  return a;
+}
+
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename V>
+__device__ __forceinline__ V* in_block(V* mine, uint32_t rank) {
+  uint64_t there;
+  asm("mapa.u64 %0, %1, %2;" : "=l"(there) : "l"((uint64_t)mine), "r"(rank));
+  return (V*)there;
+}
+
+// The finished statistics of a row: p_j = 2^{y_j - l2s}.
+struct Stats {
+  float m, M;
+  float l2s;   // log2 s; +inf in a row of nothing but -inf, NaN in one with a NaN or +inf
+  float mean;  // sum p y
+  float rest;  // sum of p outside of the teacher's entries
+  bool far;    // y from (x - m) / temperature
+  float c, inv_t;
+  __device__ bool empty() const { return l2s == kInf; }
+  __device__ float y(float x) const { return far ? (x - m) * inv_t * kLog2e : fmaf(x, c, -M); }
+  __device__ float logprob(float x) const {
+    if (empty()) return -kInf;
+    // c x may be past fp32 where the log probability is not
+    if (far || !(fabsf(x * c) <= kFar)) return (x - m) * inv_t - kLn2 * l2s;
+    return kLn2 * (y(x) - l2s);
+  }
+};
+
+// Reads back what the forward kept of a row.
+__device__ __forceinline__ Stats stats_of(const LogitsArgs& p, float m, float l2s) {
+  Stats r;
+  r.m = m;
+  r.l2s = l2s;
+  r.c = scale_of(p);
+  r.inv_t = p.inv_temperature;
+  r.far = !(fabsf(__fmul_rn(m, r.c)) <= kNear);
+  r.M = base_of(m, r.c);
+  return r;
+}
+
+// All threads of the block; `member(j)` is used with REST.
+template <typename T, bool WEIGHTED, bool REST, typename F>
+__device__ Stats finish(const LogitsArgs& p, const Row<T>& row, Sums a, F member) {
+  Stats r = stats_of(p, a.m == -kInf ? 0.f : a.m, 0.f);
+  const bool none = a.m == -kInf && !isnan(a.s);
+  if (r.far) {  // the same for every thread
+    float s = 0.f, w = 0.f, t = 0.f;
+    for (int j = threadIdx.x; j < row.V; j += kThreads) {
+      const float y = (to_f32(row.x[j]) - r.m) * r.inv_t * kLog2e, e = exp2f(y);
+      s += e;
+      if (WEIGHTED) w += e == 0.f ? 0.f : e * y;
+      if (REST && !member(j)) t += e;
+    }
+    __shared__ float part[3][kWarps];
+    float v[3] = {s, w, t};
+    for (int i = 0; i < 3; ++i) {
+      for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(~0u, v[i], o);
+      if (threadIdx.x % 32 == 0) part[i][threadIdx.x / 32] = v[i];
+    }
+    __syncthreads();
+    a.s = a.w = a.t = 0.f;
+    for (int i = 0; i < kWarps; ++i) {
+      a.s += part[0][i];
+      a.w += part[1][i];
+      a.t += part[2][i];
+    }
+  }
+  if (none || a.s == 0.f) {
+    r.l2s = kInf;
+    r.mean = r.rest = 0.f;
+  } else {
+    r.l2s = log2f(a.s);
+    r.mean = a.w / a.s;
+    r.rest = a.t / a.s;
+  }
+  return r;
+}
+
+// ---------------------------------------------------------------------------
+// The largest values of a row
+// ---------------------------------------------------------------------------
+// Order of the values (-0 as 0), then of the lower index. No value has key 0.
 __device__ __forceinline__ uint64_t order_key(float x, int j) {
   const uint32_t u = __float_as_uint(x + 0.f);
   const uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
   return (uint64_t)o << 32 | (uint32_t)~j;
 }
-
-struct RowStats {
-  float m;     // max x, or 0 in a row of nothing but -inf
-  float logs;  // log s; +inf in such a row, NaN in one with a NaN or +inf
-  float ws;    // sum e (y - m) / s
-};
-
-template <typename T>
-__device__ RowStats row_stats(const T* x, int64_t V, float inv_t) {
-  float m = -CUDART_INF_F;
-  for (int64_t j = threadIdx.x; j < V; j += blockDim.x) m = fmaxf(m, to_f32(x[j]));
-  m = block_max(m);
-  if (m == -CUDART_INF_F) m = 0.f;
-  float s = 0.f, w = 0.f;
-  for (int64_t j = threadIdx.x; j < V; j += blockDim.x) {
-    const float d = (to_f32(x[j]) - m) * inv_t, e = expf(d);
-    s += e;
-    w += e == 0.f ? 0.f : e * d;
-  }
-  s = block_sum(s);
-  w = block_sum(w);
-  if (s == 0.f) return {m, CUDART_INF_F, 0.f};
-  return {m, logf(s), w / s};
+__device__ __forceinline__ int key_index(uint64_t k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ float key_value(uint64_t k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
+// The largest value's key in each thread's vectors is known after the pass
+// that sums them. The k-th largest of 32 such keys, each the largest over one
+// lane of all warps, has k values at or above it, so only values from there up
+// can be among the k largest: some 5 for k = 5 and 130 for k = 32 in a random
+// row, found by looking at the vectors whose maximum, kept in shared memory
+// from the pass, reaches it. Keys differ even between equal values, so rows of
+// ties fill no list: lanes interleave finely, and a row of one value lists its
+// first 256 at most.
+struct TopSpace {
+  uint64_t best[kWarps][32];
+  uint64_t list[kCandidates];
+  uint64_t top[kMaxTop];
+  uint64_t floor;
+  int count;
+};
+
+// Every key >= floor of the block's part of the row goes into the list; returns their number.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p) {
-  const int64_t row = blockIdx.x;
-  const T* x = row_of<T>(p, row);
-  const RowStats r = row_stats(x, p.vocab, p.inv_temperature);
-  const bool empty = r.logs == CUDART_INF_F;
-  auto logprob = [&](int64_t j) {
-    return empty ? -CUDART_INF_F : (to_f32(x[j]) - r.m) * p.inv_temperature - r.logs;
+__device__ int collect(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles, const float* most) {
+  const float least = key_value(sp.floor);
+  auto take = [&](float x, int j) {
+    const uint64_t key = order_key(x, j);
+    if (key >= sp.floor) {
+      const int at = atomicAdd(&sp.count, 1);
+      if (at < kCandidates) sp.list[at] = key;
+    }
   };
+  for (int v = v0 + threadIdx.x; v < v1; v += kThreads)
+    if (sp.floor == 0 || most[v - v0] >= least) {
+      const uint4 raw = load_vec(row.vec(v));
+#pragma unroll
+      for (int i = 0; i < Row<T>::E / 2; ++i) {
+        const float2 f = sm100::f2_split(Vec<T>::pair(raw, i));
+        take(f.x, row.lead + v * Row<T>::E + 2 * i);
+        take(f.y, row.lead + v * Row<T>::E + 2 * i + 1);
+      }
+    }
+  if (singles && threadIdx.x < row.singles) take(to_f32(row.x[row.single(threadIdx.x)]), row.single(threadIdx.x));
+  __syncthreads();
+  return sp.count;
+}
+
+// Puts the k largest keys of list[0, n) in descending order into top; the
+// rest of top is 0.
+__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, uint64_t* top) {
+  if (threadIdx.x < kMaxTop && threadIdx.x >= min(n, k)) top[threadIdx.x] = 0;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t key = list[i];
+    int above = 0;
+    for (int j = 0; j < n; ++j) above += list[j] > key;
+    if (above < k) top[above] = key;
+  }
+  __syncthreads();
+}
+
+// The k largest keys of the block's part of the row, into sp.top. best: the
+// thread's largest maximum of a vector, at: that vector (-1: none).
+template <typename T>
+__device__ void block_top(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles, const float* most, int k,
+                          float best, int at) {
+  uint64_t key = 0;
+  if (at >= 0) {
+    const uint4 raw = load_vec(row.vec(at));
+#pragma unroll
+    for (int i = 0; i < Row<T>::E / 2; ++i) {
+      const float2 f = sm100::f2_split(Vec<T>::pair(raw, i));
+      const uint64_t a = order_key(f.x, row.lead + at * Row<T>::E + 2 * i);
+      const uint64_t b = order_key(f.y, row.lead + at * Row<T>::E + 2 * i + 1);
+      if (f.x == best && a > key) key = a;
+      if (f.y == best && b > key) key = b;
+    }
+  }
+  sp.best[threadIdx.x / 32][threadIdx.x % 32] = key;
+  if (threadIdx.x == 0) sp.count = 0;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    for (int w = 0; w < kWarps; ++w) key = sp.best[w][threadIdx.x] > key ? sp.best[w][threadIdx.x] : key;
+    int above = 0;  // lanes without a value share key 0: none of them is the k-th then, unless k reaches them
+    for (int o = 0; o < 32; ++o) {
+      const uint64_t other = __shfl_sync(~0u, key, o);
+      above += other > key || (other == key && o < threadIdx.x);
+    }
+    if (above == k - 1) sp.floor = key;
+  }
+  __syncthreads();
+  const int n = collect(sp, row, v0, v1, singles, most);
+  if (n <= kCandidates) {
+    rank_list(sp.list, n, k, sp.top);
+    return;
+  }
+  // More than the list holds (large values in few lanes): the largest below
+  // the last one found, k times over the block's part.
+  uint64_t last = ~0ull;
+  for (int i = 0; i < kMaxTop; ++i) {
+    uint64_t most_key = 0;
+    if (i < k) {
+      for (int v = v0 + threadIdx.x; v < v1; v += kThreads)
+        for (int e = 0; e < Row<T>::E; ++e) {
+          const int j = row.lead + v * Row<T>::E + e;
+          const uint64_t q = order_key(to_f32(row.x[j]), j);
+          if (q < last && q > most_key) most_key = q;
+        }
+      if (singles && threadIdx.x < row.singles) {
+        const int j = row.single(threadIdx.x);
+        const uint64_t q = order_key(to_f32(row.x[j]), j);
+        if (q < last && q > most_key) most_key = q;
+      }
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t q = __shfl_xor_sync(~0u, most_key, o);
+      most_key = q > most_key ? q : most_key;
+    }
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) sp.best[0][threadIdx.x / 32] = most_key;
+    __syncthreads();
+    for (int w = 0; w < kWarps; ++w) most_key = sp.best[0][w] > most_key ? sp.best[0][w] : most_key;
+    last = most_key;
+    if (threadIdx.x == 0) sp.top[i] = most_key;
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------
+// Token log probabilities
+// ---------------------------------------------------------------------------
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, int C) {
+  extern __shared__ float most[];  // TOP: the maximum of each of the block's vectors
+  __shared__ std::conditional_t<TOP, TopSpace, int> space;
+  __shared__ Sums peers[kMaxCluster];
+  __shared__ uint64_t peer_top[TOP ? kMaxCluster * kMaxTop : 1];
+  griddep_wait();
+  const int64_t r = blockIdx.x / C;
+  const int rank = C > 1 ? (int)sm100::cluster_ctarank() : 0;
+  if (C > 1) cluster_arrive();
+  const Row<T> row(p, r);
+  const int per = (row.vectors + C - 1) / C;
+  const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
+  Running<T, true, false> run(scale_of(p));
+  float best = -kInf;
+  int at = -1;
+  each_vectors(row, v0, v1, [&](const uint4* raw, int v, auto n) {
+    float top = -kInf;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < n) {
+        const float m = Vec<T>::max(raw[u]);
+        if constexpr (TOP) {
+          most[v + u * kThreads - v0] = m;
+          if (m > best || at < 0) {
+            best = m;
+            at = v + u * kThreads;
+          }
+        }
+        top = fmaxf(top, m);
+      }
+    run.see(top);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < n) run.add(raw[u], 0);
+  });
+  const bool singles = rank == 0;
+  if (singles && threadIdx.x < row.singles) run.add_single(to_f32(row.x[row.single(threadIdx.x)]), false);
+  Sums a = block_merge(run.sums(), run.c);
+  if constexpr (TOP) block_top(space, row, v0, v1, singles, most, p.top_k, best, at);
+  if (C > 1) {
+    cluster_wait();  // every block has begun
+    if (threadIdx.x == 0) *in_block(&peers[rank], 0) = a;
+    if constexpr (TOP)
+      if (threadIdx.x < kMaxTop) *in_block(&peer_top[rank * kMaxTop + threadIdx.x], 0) = space.top[threadIdx.x];
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+    a = peers[0];
+    for (int i = 1; i < C; ++i) a = merge(a, peers[i], run.c);
+    if constexpr (TOP) rank_list(peer_top, C * kMaxTop, p.top_k, space.top);
+  }
+  const Stats st = finish<T, true, false>(p, row, a, [](int) { return false; });
   if (threadIdx.x == 0) {
-    const int64_t t = p.targets[row];
+    const int64_t t = p.targets[r];
     float lp = 0.f;
     if (t != p.ignore_index) {
-      if (t >= 0 && t < p.vocab) {
-        lp = logprob(t);
+      if (t >= 0 && t < row.V) {
+        lp = st.logprob(to_f32(row.x[t]));
       } else {
-        lp = CUDART_NAN_F;
+        lp = kNaN;
         report_status(p.status, FAKLA_ERR_INVALID_ARG);
       }
     }
-    p.logprobs[row] = lp;
-    p.entropy[row] = empty ? 0.f : r.logs - r.ws;
+    p.logprobs[r] = lp;
+    p.entropy[r] = st.empty() ? 0.f : kLn2 * (st.l2s - st.mean);
     if (p.stats) {
-      p.stats[row * kTokenStats] = r.m;
-      p.stats[row * kTokenStats + 1] = r.logs;
+      p.stats[r * kTokenStats] = st.m;
+      p.stats[r * kTokenStats + 1] = st.l2s;
     }
   }
-  uint64_t last = ~0ull;
-  for (int k = 0; k < p.top_k; ++k) {
-    uint64_t best = 0;
-    for (int64_t j = threadIdx.x; j < p.vocab; j += blockDim.x) {
-      const uint64_t key = order_key(to_f32(x[j]), (int)j);
-      if (key < last && key > best) best = key;
+  if constexpr (TOP)
+    if (threadIdx.x < p.top_k) {
+      const uint64_t key = space.top[threadIdx.x];
+      const bool bad = isnan(st.l2s);
+      p.top_ids[r * p.top_k + threadIdx.x] = bad ? -1 : key_index(key);
+      p.top_logprobs[r * p.top_k + threadIdx.x] = bad ? kNaN : st.logprob(key_value(key));
     }
-    last = block_reduce(best, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-    if (threadIdx.x == 0) {
-      const bool bad = isnan(r.logs);
-      const int64_t j = ~(uint32_t)last;
-      p.top_ids[row * p.top_k + k] = bad ? -1 : j;
-      p.top_logprobs[row * p.top_k + k] = bad ? CUDART_NAN_F : logprob(j);
+}
+
+// ---------------------------------------------------------------------------
+// Gradients: one block per kChunk vectors of a row
+// ---------------------------------------------------------------------------
+constexpr int kChunk = kUnroll * kThreads;
+
+// Writes f(pair of logits) over a block's chunk of a row; returns the range of
+// the vectors. Stores are as wide as the loads where both rows lie alike.
+template <typename T, typename F>
+__device__ __forceinline__ void map_chunk(const Row<T>& row, T* out, int chunk, bool zero, F f) {
+  const int v0 = chunk * kChunk, v1 = min(v0 + kChunk, row.vectors);
+  const bool wide = (((uintptr_t)row.x ^ (uintptr_t)out) & 15) == 0;
+  uint4 raw[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int v = v0 + u * kThreads + threadIdx.x;
+    if (v < v1 && !zero) raw[u] = load_vec(row.vec(v));
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int v = v0 + u * kThreads + threadIdx.x;
+    if (v >= v1) continue;
+    uint4 got = make_uint4(0, 0, 0, 0);
+    if (!zero) {
+      uint64_t d[Row<T>::E / 2];
+#pragma unroll
+      for (int i = 0; i < Row<T>::E / 2; ++i) d[i] = f(raw[u], i);
+      got = Vec<T>::put(d);
+    }
+    T* to = out + row.lead + v * Row<T>::E;
+    if (wide) {
+      *reinterpret_cast<uint4*>(to) = got;
+    } else {
+      const T* e = reinterpret_cast<const T*>(&got);
+#pragma unroll
+      for (int i = 0; i < Row<T>::E; ++i) to[i] = e[i];
     }
   }
+}
+
+// Whether value j of the row is written by this chunk's block.
+template <typename T>
+__device__ __forceinline__ bool in_chunk(const Row<T>& row, int j, int chunk) {
+  const int v = row.place(j);
+  return v < 0 ? chunk == 0 : v / kChunk == chunk;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(LogitsArgs p) {
-  const int64_t row = blockIdx.x;
-  const T* x = row_of<T>(p, row);
-  T* dx = (T*)p.dlogits + row * p.vocab;
-  const float m = p.stats[row * kTokenStats], logs = p.stats[row * kTokenStats + 1];
-  const int64_t t = p.targets[row];
-  const bool counted = t != p.ignore_index;
-  float w = counted && p.dlogprobs ? p.dlogprobs[row] : 0.f;
-  if (counted && (t < 0 || t >= p.vocab)) w = CUDART_NAN_F;
-  const float h = p.dentropy ? p.dentropy[row] : 0.f, H = p.entropy[row];
+__global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(LogitsArgs p, int chunks) {
+  griddep_wait();
+  const int64_t r = blockIdx.x / chunks;
+  const int chunk = blockIdx.x % chunks;
+  const Row<T> row(p, r);
+  T* out = (T*)p.dlogits + r * p.vocab;
+  const Stats st = stats_of(p, p.stats[r * kTokenStats], p.stats[r * kTokenStats + 1]);
+  const int64_t t = p.targets[r];
+  const bool counted = t != p.ignore_index, good = t >= 0 && t < row.V;
+  float w = counted && p.dlogprobs ? p.dlogprobs[r] : 0.f;
+  if (counted && !good) w = kNaN;
+  const float h = p.dentropy ? p.dentropy[r] : 0.f;
   float total = w;
-  if (p.dtop_logprobs)
-    for (int k = 0; k < p.top_k; ++k) total += p.dtop_logprobs[row * p.top_k + k];
-  const bool empty = logs == CUDART_INF_F;
-  for (int64_t j = threadIdx.x; j < p.vocab; j += blockDim.x) {
-    const float lp = (to_f32(x[j]) - m) * p.inv_temperature - logs, e = expf(lp);
-    float dz = (counted && j == t ? w : 0.f) - total * e - (e == 0.f ? 0.f : h * e * (lp + H));
-    if (p.dtop_logprobs)
-      for (int k = 0; k < p.top_k; ++k)
-        if (p.top_ids[row * p.top_k + k] == j) dz += p.dtop_logprobs[row * p.top_k + k];
-    dx[j] = from_f32<T>(empty ? 0.f : dz * p.inv_temperature);
+  for (int k = 0; k < p.top_k; ++k) total += p.dtop_logprobs[r * p.top_k + k];
+  // dlogits_j = p_j (flat + slope log2 p_j), and what is given to j itself
+  const float flat = -(total + h * p.entropy[r]) * p.inv_temperature, slope = -h * kLn2 * p.inv_temperature;
+  auto value = [&](float x) {
+    const float l = fmaxf(st.y(x) - st.l2s, -1e30f), e = exp2_approx(st.y(x) - st.l2s);
+    return e * fmaf(l, slope, flat);
+  };
+  bool zero = st.empty() || (flat == 0.f && slope == 0.f);
+  if (st.far) {
+    const int j0 = row.lead + chunk * kChunk * Row<T>::E, j1 = row.lead + min((chunk + 1) * kChunk, row.vectors) * Row<T>::E;
+    for (int j = j0 + threadIdx.x; j < j1; j += kThreads) out[j] = from_f32<T>(zero ? 0.f : value(to_f32(row.x[j])));
+  } else {
+    const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
+    const uint64_t f2 = sm100::f2_splat(flat), s2 = sm100::f2_splat(slope);
+    const float low = -kFar / st.c;
+    auto map = [&](auto sloped) {
+      map_chunk(row, out, chunk, zero, [&](const uint4& raw, int i) {
+        uint4 v = raw;
+        if constexpr (decltype(sloped)::value) v = Vec<T>::at_least(raw, low);  // p log p is 0 there
+        const uint64_t l = sm100::f2_add(sm100::f2_fma(Vec<T>::pair(v, i), c2, nM), nl);
+        const float2 f = sm100::f2_split(l);
+        const uint64_t e = sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y)));
+        if constexpr (decltype(sloped)::value) return sm100::f2_mul(e, sm100::f2_fma(l, s2, f2));
+        else return sm100::f2_mul(e, f2);
+      });
+    };
+    if (slope == 0.f) map(std::false_type{});
+    else map(std::true_type{});
+  }
+  if (chunk == 0 && threadIdx.x < row.singles) {
+    const int j = row.single(threadIdx.x);
+    out[j] = from_f32<T>(zero ? 0.f : value(to_f32(row.x[j])));
+  }
+  if (st.empty()) return;
+  __syncthreads();
+  // the target and the alternatives once more, with their own gradients
+  if (threadIdx.x < p.top_k) {
+    const int64_t j = p.top_ids[r * p.top_k + threadIdx.x];
+    if (j >= 0 && j < row.V && in_chunk(row, (int)j, chunk)) {
+      float d = p.dtop_logprobs[r * p.top_k + threadIdx.x];
+      if (counted && j == t) d += w;
+      out[j] = from_f32<T>(fmaf(d, p.inv_temperature, value(to_f32(row.x[j]))));
+    }
+  } else if (threadIdx.x == kMaxTop && counted && good && w != 0.f && in_chunk(row, (int)t, chunk)) {
+    for (int k = 0; k < p.top_k; ++k)
+      if (p.top_ids[r * p.top_k + k] == t) return;
+    out[t] = from_f32<T>(fmaf(w, p.inv_temperature, value(to_f32(row.x[t]))));
   }
 }
 
-// The teacher's side of a row: q_k = e^{t_k / temperature - m - logs}.
+// ---------------------------------------------------------------------------
+// Distillation
+// ---------------------------------------------------------------------------
+// The teacher's side of a row: q_k = e^{t_k / temperature - m / temperature - logs}.
 struct Teacher {
   float m, logs;  // logs +inf: no distribution, every q is 0
   float mass;     // sum of the q
@@ -148,147 +690,254 @@ struct Teacher {
   bool bad;       // an id out of range
 };
 
-__device__ __forceinline__ float teacher_q(const LogitsArgs& p, int64_t row, int k, float m, float logs, float& lq) {
-  lq = -CUDART_INF_F;
-  if (p.teacher_ids[row * p.entries + k] < 0) return 0.f;
-  lq = (p.teacher_logits[row * p.entries + k] - m) * p.inv_temperature - logs;
+__device__ __forceinline__ float teacher_q(const LogitsArgs& p, int64_t id, float logit, float m, float logs, float& lq) {
+  lq = -kInf;
+  if (id < 0) return 0.f;
+  lq = (logit - m) * p.inv_temperature - logs;
   return expf(lq);
 }
 
-__device__ Teacher teacher_stats(const LogitsArgs& p, int64_t row) {
-  Teacher t = {0.f, 0.f, 0.f, 0.f, false};
-  float m = -CUDART_INF_F;
-  int bad = 0, some = 0;
-  for (int k = threadIdx.x; k < p.entries; k += blockDim.x) {
-    const int64_t id = p.teacher_ids[row * p.entries + k];
-    bad |= id < -1 || id >= p.vocab;
-    if (id < 0) continue;
-    some = 1;
-    m = fmaxf(m, p.teacher_logits[row * p.entries + k]);
+// By one warp.
+__device__ Teacher teacher_stats(const LogitsArgs& p, int64_t r) {
+  const int64_t* ids = p.teacher_ids + r * p.entries;
+  const float* logits = p.teacher_logits + r * p.entries;
+  const int lane = threadIdx.x % 32;
+  float m = -kInf;
+  bool bad = false, some = false;
+  for (int k = lane; k < p.entries; k += 32) {
+    bad |= ids[k] < -1 || ids[k] >= p.vocab;
+    some |= ids[k] >= 0;
+    if (ids[k] >= 0) m = fmaxf(m, logits[k]);
   }
-  t.bad = __syncthreads_or(bad);
-  some = __syncthreads_or(some);
-  if (p.teacher_lse) {
-    t.logs = some ? p.teacher_lse[row] : CUDART_INF_F;
-  } else {
-    m = block_max(m);
-    t.m = m == -CUDART_INF_F ? 0.f : m;
-  }
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  Teacher t;
+  t.bad = __any_sync(~0u, bad);
+  some = __any_sync(~0u, some);
+  t.m = p.teacher_lse || m == -kInf ? 0.f : m;
+  t.logs = p.teacher_lse ? (some ? p.teacher_lse[r] : kInf) : 0.f;
   float s = 0.f, lq;
-  for (int k = threadIdx.x; k < p.entries; k += blockDim.x) s += teacher_q(p, row, k, t.m, t.logs, lq);
-  s = block_sum(s);
+  for (int k = lane; k < p.entries; k += 32) s += teacher_q(p, ids[k], logits[k], t.m, t.logs, lq);
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
   if (p.teacher_lse) {
     t.mass = s;
     t.rest = some ? fmaxf(0.f, 1.f - s) : 0.f;
   } else {
-    t.logs = s == 0.f ? CUDART_INF_F : logf(s);
+    t.logs = s == 0.f ? kInf : logf(s);
     t.mass = s == 0.f ? 0.f : 1.f;
+    t.rest = 0.f;
   }
   return t;
 }
 
-__device__ bool is_member(const LogitsArgs& p, int64_t row, int64_t j) {
-  for (int k = 0; k < p.entries; ++k)
-    if (p.teacher_ids[row * p.entries + k] == j) return true;
-  return false;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p) {
-  const int64_t row = blockIdx.x;
-  const T* x = row_of<T>(p, row);
-  const RowStats r = row_stats(x, p.vocab, p.inv_temperature);
-  const Teacher t = teacher_stats(p, row);
-  auto logprob = [&](int64_t j) {
-    return r.logs == CUDART_INF_F ? -CUDART_INF_F : (to_f32(x[j]) - r.m) * p.inv_temperature - r.logs;
-  };
+// REST: teacher_lse is given, and the sum outside of the entries is needed on
+// its own (1 - sum p_k would cancel): one byte per vector says which of its
+// values are entries.
+template <typename T, bool REST>
+__global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) {
+  extern __shared__ uint32_t marks[];
+  __shared__ uint32_t single_marks;
+  __shared__ Sums peers[kMaxCluster];
+  griddep_wait();
+  const int64_t r = blockIdx.x / C;
+  const int rank = C > 1 ? (int)sm100::cluster_ctarank() : 0;
+  if (C > 1) cluster_arrive();
+  const Row<T> row(p, r);
+  const int per = (row.vectors + C - 1) / C;
+  const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
+  const int64_t* ids = p.teacher_ids + r * p.entries;
+  if constexpr (REST) {
+    for (int i = threadIdx.x; i < (v1 - v0 + 3) / 4; i += kThreads) marks[i] = 0;
+    if (threadIdx.x == 0) single_marks = 0;
+    __syncthreads();
+    if (threadIdx.x < p.entries) {
+      const int64_t id = ids[threadIdx.x];
+      if (id >= 0 && id < row.V) {
+        const int v = row.place((int)id);
+        if (v < 0) atomicOr(&single_marks, 1u << (-1 - v));
+        else if (v >= v0 && v < v1) atomicOr(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + ((int)id - row.lead) % Row<T>::E));
+      }
+    }
+    __syncthreads();
+  }
+  Running<T, false, REST> run(scale_of(p));
+  const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
+  each_vectors(row, v0, v1, [&](const uint4* raw, int v, auto n) {
+    float top = -kInf;
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < n) top = fmaxf(top, Vec<T>::max(raw[u]));
+    run.see(top);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (u < n) run.add(raw[u], REST ? mark[v + u * kThreads - v0] : 0);
+  });
+  if (rank == 0 && threadIdx.x < row.singles)
+    run.add_single(to_f32(row.x[row.single(threadIdx.x)]), REST && (single_marks >> threadIdx.x & 1));
+  Sums a = block_merge(run.sums(), run.c);
+  if (C > 1) {
+    cluster_wait();
+    if (threadIdx.x == 0) *in_block(&peers[rank], 0) = a;
+    cluster_arrive();
+    cluster_wait();
+    if (rank != 0) return;
+    a = peers[0];
+    for (int i = 1; i < C; ++i) a = merge(a, peers[i], run.c);
+  }
+  const Stats st = finish<T, false, REST>(p, row, a, [&](int j) {
+    for (int k = 0; k < p.entries; ++k)
+      if (ids[k] == j) return true;
+    return false;
+  });
+  if (threadIdx.x >= 32) return;
+  const Teacher t = teacher_stats(p, r);
   float loss = 0.f;
   if (!t.bad)
-    for (int k = threadIdx.x; k < p.entries; k += blockDim.x) {
+    for (int k = threadIdx.x; k < p.entries; k += 32) {
       float lq;
-      const float q = teacher_q(p, row, k, t.m, t.logs, lq);
-      if (q != 0.f) loss += q * (lq - logprob(p.teacher_ids[row * p.entries + k]));
+      const float q = teacher_q(p, ids[k], p.teacher_logits[r * p.entries + k], t.m, t.logs, lq);
+      if (q != 0.f) loss += q * (lq - st.logprob(to_f32(row.x[ids[k]])));
     }
-  loss = block_sum(loss);
+  for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(~0u, loss, o);
   float ratio = 0.f;  // q_r / p_r
-  if (p.teacher_lse && !t.bad) {
-    float s = 0.f;
-    for (int64_t j = threadIdx.x; j < p.vocab; j += blockDim.x)
-      if (!is_member(p, row, j)) s += expf((to_f32(x[j]) - r.m) * p.inv_temperature - r.logs);
-    s = block_sum(s);
-    if (t.rest > 0.f) {
-      ratio = t.rest / s;
-      loss += t.rest * logf(ratio);
-    }
+  if (REST && t.rest > 0.f) {
+    ratio = t.rest / st.rest;
+    loss += t.rest * logf(ratio);
   }
   if (threadIdx.x != 0) return;
   if (t.bad) {
-    loss = CUDART_NAN_F;
+    loss = kNaN;
     report_status(p.status, FAKLA_ERR_INVALID_ARG);
   }
-  p.loss[row] = loss;
+  p.loss[r] = loss;
   if (p.stats) {
-    float* st = p.stats + row * kDistillStats;
-    st[0] = r.m;
-    st[1] = r.logs;
-    st[2] = t.m;
-    st[3] = t.logs;
-    st[4] = t.bad ? CUDART_NAN_F : t.mass + t.rest;
-    st[5] = ratio;
+    float* keep = p.stats + r * kDistillStats;
+    keep[0] = st.m;
+    keep[1] = st.l2s;
+    keep[2] = t.m;
+    keep[3] = t.logs;
+    keep[4] = t.bad ? kNaN : t.mass + t.rest;
+    keep[5] = isinf(ratio) ? 0.f : ratio;  // infinite: every p outside of the entries is 0
   }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p) {
-  const int64_t row = blockIdx.x;
-  const T* x = row_of<T>(p, row);
-  T* dx = (T*)p.dlogits + row * p.vocab;
-  const float* st = p.stats + row * kDistillStats;
-  const float g = p.dloss[row] * p.inv_temperature;
-  const bool empty = st[1] == CUDART_INF_F;
-  for (int64_t j = threadIdx.x; j < p.vocab; j += blockDim.x) {
-    const float e = empty ? 0.f : expf((to_f32(x[j]) - st[0]) * p.inv_temperature - st[1]);
-    float dz = e * st[4];
-    bool member = false;
-    for (int k = 0; k < p.entries; ++k)
-      if (p.teacher_ids[row * p.entries + k] == j) {
-        float lq;
-        dz -= empty ? 0.f : teacher_q(p, row, k, st[2], st[3], lq);
-        member = true;
-      }
-    if (!member && e != 0.f) dz -= e * st[5];
-    dx[j] = from_f32<T>(dz * g);
+__global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p, int chunks) {
+  __shared__ int id_of[kMaxEntries];
+  __shared__ float q_of[kMaxEntries];
+  griddep_wait();
+  const int64_t r = blockIdx.x / chunks;
+  const int chunk = blockIdx.x % chunks;
+  const Row<T> row(p, r);
+  T* out = (T*)p.dlogits + r * p.vocab;
+  const float* keep = p.stats + r * kDistillStats;
+  const Stats st = stats_of(p, keep[0], keep[1]);
+  const float g = p.dloss[r] * p.inv_temperature;
+  // dlogits_j = p_j outer, or for an entry p_j inner - its q
+  const float inner = keep[4] * g, outer = (keep[4] - keep[5]) * g;
+  if (threadIdx.x < p.entries) {
+    const int64_t id = p.teacher_ids[r * p.entries + threadIdx.x];
+    float lq;
+    q_of[threadIdx.x] = teacher_q(p, id, p.teacher_logits[r * p.entries + threadIdx.x], keep[2], keep[3], lq);
+    id_of[threadIdx.x] = id >= 0 && id < row.V ? (int)id : -1;
   }
+  auto prob = [&](float x) { return exp2_approx(st.y(x) - st.l2s); };
+  const bool zero = g == 0.f || (st.empty() && !isnan(inner));
+  if (st.far) {
+    const int j0 = row.lead + chunk * kChunk * Row<T>::E, j1 = row.lead + min((chunk + 1) * kChunk, row.vectors) * Row<T>::E;
+    for (int j = j0 + threadIdx.x; j < j1; j += kThreads) out[j] = from_f32<T>(zero ? 0.f : prob(to_f32(row.x[j])) * outer);
+  } else {
+    const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
+    const uint64_t o2 = sm100::f2_splat(outer);
+    map_chunk(row, out, chunk, zero, [&](const uint4& raw, int i) {
+      const float2 f = sm100::f2_split(sm100::f2_add(sm100::f2_fma(Vec<T>::pair(raw, i), c2, nM), nl));
+      return sm100::f2_mul(sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y))), o2);
+    });
+  }
+  if (chunk == 0 && threadIdx.x < row.singles) {
+    const int j = row.single(threadIdx.x);
+    out[j] = from_f32<T>(zero ? 0.f : prob(to_f32(row.x[j])) * outer);
+  }
+  if (zero) return;
+  __syncthreads();
+  // the entries once more, each by the first that names it
+  if (threadIdx.x >= p.entries) return;
+  const int j = id_of[threadIdx.x];
+  if (j < 0 || !in_chunk(row, j, chunk)) return;
+  float q = 0.f;
+  for (int k = 0; k < p.entries; ++k)
+    if (id_of[k] == j) {
+      if (k < threadIdx.x) return;
+      q += q_of[k];
+    }
+  out[j] = from_f32<T>(prob(to_f32(row.x[j])) * inner - q * g);
+}
+
+// ---------------------------------------------------------------------------
+// Launches
+// ---------------------------------------------------------------------------
+// Blocks of a cluster, which share a row: as many as give every SM two blocks,
+// while each keeps a full round of loads, and as a block's shared memory asks
+// for (`bytes` per vector).
+int cluster_size(int64_t rows, int64_t vectors, int bytes) {
+  int c = 1;
+  while (c < kMaxCluster && ((rows * c < 2 * fakla_sm_count() && vectors / (2 * c) >= kThreads) ||
+                             vectors / c * bytes > (48 << 10)))
+    c *= 2;
+  return c;
+}
+
+template <typename K>
+cudaError_t launch_rows(K kernel, const LogitsArgs& p, int per_vector, int bytes, cudaStream_t stream) {
+  const int64_t vectors = p.vocab / per_vector;
+  const int c = cluster_size(p.batch * p.rows, vectors, bytes);
+  const size_t smem = ((size_t)((vectors + c - 1) / c + 1) * bytes + 15) / 16 * 16;
+  if (smem > (32 << 10)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  return launch_chained(kernel, dim3((unsigned)(p.batch * p.rows * c)), dim3(kThreads), smem, stream, (unsigned)c, p, c);
+}
+
+template <typename K>
+cudaError_t launch_chunks(K kernel, const LogitsArgs& p, int per_vector, cudaStream_t stream) {
+  const int chunks = (int)((p.vocab / per_vector + kChunk - 1) / kChunk);
+  const int n = chunks > 0 ? chunks : 1;
+  return launch_chained(kernel, dim3((unsigned)(p.batch * p.rows * n)), dim3(kThreads), 0, stream, 1u, p, n);
+}
+
+template <typename F>
+cudaError_t by_type(int dtype, F f) {
+  return dtype == FAKLA_BF16 ? f(__nv_bfloat16{}) : f(float{});
 }
 
 }  // namespace
 
 cudaError_t launch_token_logprobs(int dtype, const LogitsArgs& p, cudaStream_t stream) {
-  const unsigned grid = (unsigned)(p.batch * p.rows);
-  if (dtype == FAKLA_BF16) token_logprobs_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p);
-  else token_logprobs_kernel<float><<<grid, kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return by_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (p.top_k > 0) return launch_rows(token_logprobs_kernel<T, true>, p, Vec<T>::E, (int)sizeof(float), stream);
+    return launch_rows(token_logprobs_kernel<T, false>, p, Vec<T>::E, 0, stream);
+  });
 }
 
 cudaError_t launch_token_logprobs_backward(int dtype, const LogitsArgs& p, cudaStream_t stream) {
-  const unsigned grid = (unsigned)(p.batch * p.rows);
-  if (dtype == FAKLA_BF16) token_logprobs_backward_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p);
-  else token_logprobs_backward_kernel<float><<<grid, kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return by_type(dtype, [&](auto t) {
+    return launch_chunks(token_logprobs_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
+  });
 }
 
 cudaError_t launch_distill(int dtype, const LogitsArgs& p, cudaStream_t stream) {
-  const unsigned grid = (unsigned)(p.batch * p.rows);
-  if (dtype == FAKLA_BF16) distill_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p);
-  else distill_kernel<float><<<grid, kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return by_type(dtype, [&](auto t) {
+    typedef decltype(t) T;
+    if (p.teacher_lse) return launch_rows(distill_kernel<T, true>, p, Vec<T>::E, 1, stream);
+    return launch_rows(distill_kernel<T, false>, p, Vec<T>::E, 0, stream);
+  });
 }
 
 cudaError_t launch_distill_backward(int dtype, const LogitsArgs& p, cudaStream_t stream) {
-  const unsigned grid = (unsigned)(p.batch * p.rows);
-  if (dtype == FAKLA_BF16) distill_backward_kernel<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(p);
-  else distill_backward_kernel<float><<<grid, kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return by_type(dtype, [&](auto t) {
+    return launch_chunks(distill_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
+  });
 }
 
 }  // namespace fakla
