@@ -32,12 +32,15 @@
 namespace fakla {
 namespace {
 
-constexpr int kThreads = 256;
+// Few threads to a row: what each does once (its place, the merge of its sums)
+// is spread over more values. With 256, 32000 bf16 values per row cost 13
+// instructions each and 76 us for 4096 rows.
+constexpr int kThreads = 128;
 constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;      // 16-byte loads of a thread in flight
 constexpr int kMaxCluster = 8;  // the largest portable cluster
 constexpr int kMaxTop = 32;     // as fakla_token_logprobs takes; also the lanes of a warp
-constexpr int kMaxEntries = kThreads;
+constexpr int kMaxEntries = 256;  // as fakla_distill_topk takes
 constexpr int kCandidates = 1024;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kNaN = __builtin_nanf("");
@@ -116,8 +119,9 @@ struct Row {
   static constexpr int E = Vec<T>::E;
   const T* x;
   int V, lead, vectors, singles;
-  __device__ Row(const LogitsArgs& p, int64_t row) {
-    x = (const T*)p.logits + row / p.rows * p.batch_stride + row % p.rows * p.row_stride;
+  __device__ Row(const LogitsArgs& p, uint32_t row) {
+    const uint32_t rows = (uint32_t)p.rows, i = p.batch == 1 ? 0 : row / rows;
+    x = (const T*)p.logits + i * p.batch_stride + (row - i * rows) * p.row_stride;
     V = (int)p.vocab;
     lead = (int)(-(intptr_t)x & 15) / (int)sizeof(T);
     if (lead > V) lead = V;
@@ -147,18 +151,23 @@ struct Sums {
 // M of a maximum m, kept finite for -inf.
 __device__ __forceinline__ float base_of(float m, float c) { return fmaxf(__fmul_rn(m, c), -kFar); }
 
-__device__ __forceinline__ void move_base(Sums& a, float from, float to) {
-  const float f = exp2_approx(from - to);
-  a.w = f * fmaf(from - to, a.s, a.w);
+// The sums over `width` neighbouring lanes (a power of two), in each of them:
+// all are moved to the largest value's base once, then added in a fixed order.
+template <bool WEIGHTED, bool REST>
+__device__ __forceinline__ Sums merge_lanes(Sums a, float c, int width) {
+  float m = a.m;
+  for (int o = width / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  const float move = base_of(a.m, c) - base_of(m, c), f = exp2_approx(move);
+  if (WEIGHTED) a.w = f * fmaf(move, a.s, a.w);
   a.s *= f;
-  a.t *= f;
-}
-
-__device__ __forceinline__ Sums merge(Sums a, Sums b, float c) {
-  const float A = base_of(a.m, c), B = base_of(b.m, c);
-  if (A >= B) move_base(b, B, A);
-  else move_base(a, A, B);
-  return {fmaxf(a.m, b.m), a.s + b.s, a.w + b.w, a.t + b.t};
+  if (REST) a.t *= f;
+  for (int o = width / 2; o > 0; o >>= 1) {
+    a.s += __shfl_xor_sync(~0u, a.s, o);
+    if (WEIGHTED) a.w += __shfl_xor_sync(~0u, a.w, o);
+    if (REST) a.t += __shfl_xor_sync(~0u, a.t, o);
+  }
+  a.m = m;
+  return a;
 }
 
 // One thread's running sums. WEIGHTED: the entropy's; REST: those outside of
@@ -222,47 +231,42 @@ struct Running {
   }
 };
 
-// A number of vectors known when compiling.
-template <int N>
-struct Count {
-  __device__ constexpr operator int() const { return N; }
-};
-
-// Runs f(vectors, the first one's number, how many) on every thread's vectors
-// of [v0, v1), kUnroll at a time, kThreads apart.
+// Runs f(vectors, the first one's number) on every thread's vectors of
+// [v0, v1), kUnroll at a time, kThreads apart; the next ones are on their way
+// meanwhile. Past v1 the values are -inf, which add nothing.
 template <typename T, typename F>
 __device__ __forceinline__ void each_vectors(const Row<T>& row, int v0, int v1, F f) {
-  for (int v = v0 + threadIdx.x; v < v1; v += kUnroll * kThreads) {
-    uint4 raw[kUnroll];
-    const int n = (v1 - v + kThreads - 1) / kThreads;
-    if (n >= kUnroll) {
+  auto fetch = [&](uint4* raw, int v) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) raw[u] = load_vec(row.vec(v + u * kThreads));
-      f(raw, v, Count<kUnroll>{});
-    } else {
-#pragma unroll
-      for (int u = 0; u < kUnroll - 1; ++u)
-        if (u < n) raw[u] = load_vec(row.vec(v + u * kThreads));
-      f(raw, v, n);
+    for (int u = 0; u < kUnroll; ++u) {
+      constexpr uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+      raw[u] = make_uint4(none, none, none, none);
+      if (v + u * kThreads < v1) raw[u] = load_vec(row.vec(v + u * kThreads));
     }
+  };
+  constexpr int step = kUnroll * kThreads;
+  uint4 even[kUnroll], odd[kUnroll];
+  int v = v0 + threadIdx.x;
+  fetch(even, v);
+  while (v < v1) {
+    fetch(odd, v + step);
+    f(even, v);
+    v += step;
+    if (v >= v1) break;
+    fetch(even, v + step);
+    f(odd, v);
+    v += step;
   }
 }
 
-__device__ Sums block_merge(Sums a, float c) {
+// The sums over the block, in every thread.
+template <bool WEIGHTED, bool REST>
+__device__ __forceinline__ Sums merge_block(Sums a, float c) {
   __shared__ Sums part[kWarps];
-  auto from = [&](int o) {
-    return Sums{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.w, o),
-                __shfl_xor_sync(~0u, a.t, o)};
-  };
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums b = from(o);
-    a = threadIdx.x & o ? merge(b, a, c) : merge(a, b, c);
-  }
+  a = merge_lanes<WEIGHTED, REST>(a, c, 32);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = a;
   __syncthreads();
-  a = part[0];
-  for (int i = 1; i < kWarps; ++i) a = merge(a, part[i], c);
-  return a;
+  return merge_lanes<WEIGHTED, REST>(part[threadIdx.x % kWarps], c, kWarps);
 }
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -368,40 +372,47 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 // that sums them. The k-th largest of 32 such keys, each the largest over one
 // lane of all warps, has k values at or above it, so only values from there up
 // can be among the k largest: some 5 for k = 5 and 130 for k = 32 in a random
-// row, found by looking at the vectors whose maximum, kept in shared memory
-// from the pass, reaches it. Keys differ even between equal values, so rows of
-// ties fill no list: lanes interleave finely, and a row of one value lists its
-// first 256 at most.
+// row. They are in the vectors whose maximum, kept in shared memory from the
+// pass, reaches it; those are listed first and then read again all at once, by
+// a thread per value. Keys differ even between equal values, so rows of ties
+// fill no list: lanes interleave finely, and a row of one value lists its first
+// 256 at most.
 struct TopSpace {
   uint64_t best[kWarps][32];
   uint64_t list[kCandidates];
+  int vectors[kCandidates];
   uint64_t top[kMaxTop];
   uint64_t floor;
-  int count;
+  int vector_count, count;
 };
 
-// Every key >= floor of the block's part of the row goes into the list; returns their number.
+// Every key >= floor of the block's part of the row goes into the list; returns
+// their number, more than kCandidates if that or their vectors are too many.
 template <typename T>
-__device__ int collect(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles, const float* most) {
-  const float least = key_value(sp.floor);
-  auto take = [&](float x, int j) {
-    const uint64_t key = order_key(x, j);
-    if (key >= sp.floor) {
+__device__ __forceinline__ int collect(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles,
+                                       const float* most) {
+  constexpr int E = Row<T>::E;
+  const uint64_t floor = sp.floor;
+  const float least = floor == 0 ? -kInf : key_value(floor);
+  // equal maxima count up to the vector of the floor's own index
+  const int last = floor == 0 ? v1 : (key_index(floor) - row.lead) / E;
+  for (int v = v0 + threadIdx.x; v < v1; v += kThreads)
+    if (most[v - v0] > least || (most[v - v0] == least && v <= last)) {
+      const int at = atomicAdd(&sp.vector_count, 1);
+      if (at < kCandidates) sp.vectors[at] = v;
+    }
+  __syncthreads();
+  const int n = sp.vector_count;
+  if (n > kCandidates) return n;
+  auto take = [&](int j) {
+    const uint64_t key = order_key(to_f32(row.x[j]), j);
+    if (key >= floor) {
       const int at = atomicAdd(&sp.count, 1);
       if (at < kCandidates) sp.list[at] = key;
     }
   };
-  for (int v = v0 + threadIdx.x; v < v1; v += kThreads)
-    if (sp.floor == 0 || most[v - v0] >= least) {
-      const uint4 raw = load_vec(row.vec(v));
-#pragma unroll
-      for (int i = 0; i < Row<T>::E / 2; ++i) {
-        const float2 f = sm100::f2_split(Vec<T>::pair(raw, i));
-        take(f.x, row.lead + v * Row<T>::E + 2 * i);
-        take(f.y, row.lead + v * Row<T>::E + 2 * i + 1);
-      }
-    }
-  if (singles && threadIdx.x < row.singles) take(to_f32(row.x[row.single(threadIdx.x)]), row.single(threadIdx.x));
+  for (int i = threadIdx.x; i < n * E; i += kThreads) take(row.lead + sp.vectors[i / E] * E + i % E);
+  if (singles && threadIdx.x < row.singles) take(row.single(threadIdx.x));
   __syncthreads();
   return sp.count;
 }
@@ -413,6 +424,7 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, ui
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t key = list[i];
     int above = 0;
+#pragma unroll 8
     for (int j = 0; j < n; ++j) above += list[j] > key;
     if (above < k) top[above] = key;
   }
@@ -420,28 +432,28 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, ui
 }
 
 // The k largest keys of the block's part of the row, into sp.top. best: the
-// thread's largest maximum of a vector, at: that vector (-1: none).
+// thread's vector with the largest maximum, at: its number (-1: none).
 template <typename T>
-__device__ void block_top(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles, const float* most, int k,
-                          float best, int at) {
+__device__ __forceinline__ void block_top(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles,
+                                          const float* most, int k, const uint4& best, int at) {
   uint64_t key = 0;
   if (at >= 0) {
-    const uint4 raw = load_vec(row.vec(at));
+    const float m = Vec<T>::max(best);
 #pragma unroll
-    for (int i = 0; i < Row<T>::E / 2; ++i) {
-      const float2 f = sm100::f2_split(Vec<T>::pair(raw, i));
-      const uint64_t a = order_key(f.x, row.lead + at * Row<T>::E + 2 * i);
-      const uint64_t b = order_key(f.y, row.lead + at * Row<T>::E + 2 * i + 1);
-      if (f.x == best && a > key) key = a;
-      if (f.y == best && b > key) key = b;
+    for (int i = Row<T>::E / 2 - 1; i >= 0; --i) {
+      const float2 f = sm100::f2_split(Vec<T>::pair(best, i));
+      const int j = row.lead + at * Row<T>::E + 2 * i;
+      if (f.y == m) key = order_key(f.y, j + 1);
+      if (f.x == m) key = order_key(f.x, j);
     }
   }
   sp.best[threadIdx.x / 32][threadIdx.x % 32] = key;
-  if (threadIdx.x == 0) sp.count = 0;
+  if (threadIdx.x == 0) sp.count = sp.vector_count = 0;
   __syncthreads();
   if (threadIdx.x < 32) {
     for (int w = 0; w < kWarps; ++w) key = sp.best[w][threadIdx.x] > key ? sp.best[w][threadIdx.x] : key;
-    int above = 0;  // lanes without a value share key 0: none of them is the k-th then, unless k reaches them
+    int above = 0;  // its rank among the lanes; those without a value share key 0, in the order of the lanes
+#pragma unroll
     for (int o = 0; o < 32; ++o) {
       const uint64_t other = __shfl_sync(~0u, key, o);
       above += other > key || (other == key && o < threadIdx.x);
@@ -454,6 +466,7 @@ __device__ void block_top(TopSpace& sp, const Row<T>& row, int v0, int v1, bool 
     rank_list(sp.list, n, k, sp.top);
     return;
   }
+  __syncthreads();
   // More than the list holds (large values in few lanes): the largest below
   // the last one found, k times over the block's part.
   uint64_t last = ~0ull;
@@ -496,38 +509,40 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
   __shared__ Sums peers[kMaxCluster];
   __shared__ uint64_t peer_top[TOP ? kMaxCluster * kMaxTop : 1];
   griddep_wait();
-  const int64_t r = blockIdx.x / C;
+  const uint32_t r = blockIdx.x / C;
   const int rank = C > 1 ? (int)sm100::cluster_ctarank() : 0;
   if (C > 1) cluster_arrive();
   const Row<T> row(p, r);
   const int per = (row.vectors + C - 1) / C;
   const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
   Running<T, true, false> run(scale_of(p));
-  float best = -kInf;
+  float best_max = -kInf;
+  uint4 best = make_uint4(0, 0, 0, 0);
   int at = -1;
-  each_vectors(row, v0, v1, [&](const uint4* raw, int v, auto n) {
+  const int64_t t = rank == 0 && threadIdx.x == 0 ? p.targets[r] : -1;
+  each_vectors(row, v0, v1, [&](const uint4* raw, int v) {
     float top = -kInf;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (u < n) {
-        const float m = Vec<T>::max(raw[u]);
-        if constexpr (TOP) {
-          most[v + u * kThreads - v0] = m;
-          if (m > best || at < 0) {
-            best = m;
-            at = v + u * kThreads;
-          }
+    for (int u = 0; u < kUnroll; ++u) {
+      const float m = Vec<T>::max(raw[u]);
+      if (TOP && v + u * kThreads < v1) {
+        most[v + u * kThreads - v0] = m;
+        if (m > best_max || at < 0) {
+          best_max = m;
+          best = raw[u];
+          at = v + u * kThreads;
         }
-        top = fmaxf(top, m);
       }
+      top = fmaxf(top, m);
+    }
     run.see(top);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (u < n) run.add(raw[u], 0);
+    for (int u = 0; u < kUnroll; ++u) run.add(raw[u], 0);
   });
   const bool singles = rank == 0;
   if (singles && threadIdx.x < row.singles) run.add_single(to_f32(row.x[row.single(threadIdx.x)]), false);
-  Sums a = block_merge(run.sums(), run.c);
+  const float target = t >= 0 && t < row.V ? to_f32(row.x[t]) : 0.f;
+  Sums a = merge_block<true, false>(run.sums(), run.c);
   if constexpr (TOP) block_top(space, row, v0, v1, singles, most, p.top_k, best, at);
   if (C > 1) {
     cluster_wait();  // every block has begun
@@ -537,17 +552,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    a = peers[0];
-    for (int i = 1; i < C; ++i) a = merge(a, peers[i], run.c);
+    a = merge_lanes<true, false>(peers[threadIdx.x % C], run.c, C);
     if constexpr (TOP) rank_list(peer_top, C * kMaxTop, p.top_k, space.top);
   }
   const Stats st = finish<T, true, false>(p, row, a, [](int) { return false; });
   if (threadIdx.x == 0) {
-    const int64_t t = p.targets[r];
     float lp = 0.f;
     if (t != p.ignore_index) {
       if (t >= 0 && t < row.V) {
-        lp = st.logprob(to_f32(row.x[t]));
+        lp = st.logprob(target);
       } else {
         lp = kNaN;
         report_status(p.status, FAKLA_ERR_INVALID_ARG);
@@ -556,80 +569,78 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
     p.logprobs[r] = lp;
     p.entropy[r] = st.empty() ? 0.f : kLn2 * (st.l2s - st.mean);
     if (p.stats) {
-      p.stats[r * kTokenStats] = st.m;
-      p.stats[r * kTokenStats + 1] = st.l2s;
+      p.stats[(int64_t)r * kTokenStats] = st.m;
+      p.stats[(int64_t)r * kTokenStats + 1] = st.l2s;
     }
   }
   if constexpr (TOP)
     if (threadIdx.x < p.top_k) {
       const uint64_t key = space.top[threadIdx.x];
       const bool bad = isnan(st.l2s);
-      p.top_ids[r * p.top_k + threadIdx.x] = bad ? -1 : key_index(key);
-      p.top_logprobs[r * p.top_k + threadIdx.x] = bad ? kNaN : st.logprob(key_value(key));
+      p.top_ids[(int64_t)r * p.top_k + threadIdx.x] = bad ? -1 : key_index(key);
+      p.top_logprobs[(int64_t)r * p.top_k + threadIdx.x] = bad ? kNaN : st.logprob(key_value(key));
     }
 }
 
 // ---------------------------------------------------------------------------
-// Gradients: one block per kChunk vectors of a row
+// Gradients: one block per `span` vectors of a row
 // ---------------------------------------------------------------------------
-constexpr int kChunk = kUnroll * kThreads;
+constexpr int kRound = kUnroll * kThreads;  // vectors of a block's loads in flight
 
-// Writes f(pair of logits) over a block's chunk of a row; returns the range of
-// the vectors. Stores are as wide as the loads where both rows lie alike.
+// Writes f(pair of logits) over the block's vectors [v0, v1) of a row. Stores
+// are as wide as the loads where both rows lie alike.
 template <typename T, typename F>
-__device__ __forceinline__ void map_chunk(const Row<T>& row, T* out, int chunk, bool zero, F f) {
-  const int v0 = chunk * kChunk, v1 = min(v0 + kChunk, row.vectors);
+__device__ __forceinline__ void map_vectors(const Row<T>& row, T* out, int v0, int v1, bool zero, F f) {
   const bool wide = (((uintptr_t)row.x ^ (uintptr_t)out) & 15) == 0;
-  uint4 raw[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int v = v0 + u * kThreads + threadIdx.x;
-    if (v < v1 && !zero) raw[u] = load_vec(row.vec(v));
-  }
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int v = v0 + u * kThreads + threadIdx.x;
-    if (v >= v1) continue;
-    uint4 got = make_uint4(0, 0, 0, 0);
-    if (!zero) {
-      uint64_t d[Row<T>::E / 2];
-#pragma unroll
-      for (int i = 0; i < Row<T>::E / 2; ++i) d[i] = f(raw[u], i);
-      got = Vec<T>::put(d);
-    }
+  auto put = [&](uint4 got, int v) {
     T* to = out + row.lead + v * Row<T>::E;
     if (wide) {
-      *reinterpret_cast<uint4*>(to) = got;
+      __stcs(reinterpret_cast<uint4*>(to), got);
     } else {
       const T* e = reinterpret_cast<const T*>(&got);
 #pragma unroll
       for (int i = 0; i < Row<T>::E; ++i) to[i] = e[i];
     }
+  };
+  if (zero) {
+    for (int v = v0 + threadIdx.x; v < v1; v += kThreads) put(make_uint4(0, 0, 0, 0), v);
+    return;
   }
+  each_vectors(row, v0, v1, [&](const uint4* raw, int v) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+      if (v + u * kThreads < v1) {
+        uint64_t d[Row<T>::E / 2];
+#pragma unroll
+        for (int i = 0; i < Row<T>::E / 2; ++i) d[i] = f(raw[u], i);
+        put(Vec<T>::put(d), v + u * kThreads);
+      }
+  });
 }
 
-// Whether value j of the row is written by this chunk's block.
+// Whether value j of the row is written by the block of vectors [v0, v1).
 template <typename T>
-__device__ __forceinline__ bool in_chunk(const Row<T>& row, int j, int chunk) {
+__device__ __forceinline__ bool writes(const Row<T>& row, int j, int chunk, int v0, int v1) {
   const int v = row.place(j);
-  return v < 0 ? chunk == 0 : v / kChunk == chunk;
+  return v < 0 ? chunk == 0 : v >= v0 && v < v1;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(LogitsArgs p, int chunks) {
+__global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(LogitsArgs p, int chunks, int span) {
   griddep_wait();
-  const int64_t r = blockIdx.x / chunks;
-  const int chunk = blockIdx.x % chunks;
+  const uint32_t r = blockIdx.x / chunks;
+  const int chunk = blockIdx.x - r * chunks;
   const Row<T> row(p, r);
-  T* out = (T*)p.dlogits + r * p.vocab;
-  const Stats st = stats_of(p, p.stats[r * kTokenStats], p.stats[r * kTokenStats + 1]);
+  const int v0 = min(chunk * span, row.vectors), v1 = min(v0 + span, row.vectors);
+  T* out = (T*)p.dlogits + (int64_t)r * p.vocab;
+  const Stats st = stats_of(p, p.stats[(int64_t)r * kTokenStats], p.stats[(int64_t)r * kTokenStats + 1]);
   const int64_t t = p.targets[r];
   const bool counted = t != p.ignore_index, good = t >= 0 && t < row.V;
   float w = counted && p.dlogprobs ? p.dlogprobs[r] : 0.f;
   if (counted && !good) w = kNaN;
   const float h = p.dentropy ? p.dentropy[r] : 0.f;
   float total = w;
-  for (int k = 0; k < p.top_k; ++k) total += p.dtop_logprobs[r * p.top_k + k];
+  for (int k = 0; k < p.top_k; ++k) total += p.dtop_logprobs[(int64_t)r * p.top_k + k];
   // dlogits_j = p_j (flat + slope log2 p_j), and what is given to j itself
   const float flat = -(total + h * p.entropy[r]) * p.inv_temperature, slope = -h * kLn2 * p.inv_temperature;
   auto value = [&](float x) {
@@ -638,14 +649,14 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
   };
   bool zero = st.empty() || (flat == 0.f && slope == 0.f);
   if (st.far) {
-    const int j0 = row.lead + chunk * kChunk * Row<T>::E, j1 = row.lead + min((chunk + 1) * kChunk, row.vectors) * Row<T>::E;
-    for (int j = j0 + threadIdx.x; j < j1; j += kThreads) out[j] = from_f32<T>(zero ? 0.f : value(to_f32(row.x[j])));
+    for (int j = row.lead + v0 * Row<T>::E + threadIdx.x; j < row.lead + v1 * Row<T>::E; j += kThreads)
+      out[j] = from_f32<T>(zero ? 0.f : value(to_f32(row.x[j])));
   } else {
     const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
     const uint64_t f2 = sm100::f2_splat(flat), s2 = sm100::f2_splat(slope);
     const float low = -kFar / st.c;
     auto map = [&](auto sloped) {
-      map_chunk(row, out, chunk, zero, [&](const uint4& raw, int i) {
+      map_vectors(row, out, v0, v1, zero, [&](const uint4& raw, int i) {
         uint4 v = raw;
         if constexpr (decltype(sloped)::value) v = Vec<T>::at_least(raw, low);  // p log p is 0 there
         const uint64_t l = sm100::f2_add(sm100::f2_fma(Vec<T>::pair(v, i), c2, nM), nl);
@@ -666,15 +677,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
   __syncthreads();
   // the target and the alternatives once more, with their own gradients
   if (threadIdx.x < p.top_k) {
-    const int64_t j = p.top_ids[r * p.top_k + threadIdx.x];
-    if (j >= 0 && j < row.V && in_chunk(row, (int)j, chunk)) {
-      float d = p.dtop_logprobs[r * p.top_k + threadIdx.x];
+    const int64_t j = p.top_ids[(int64_t)r * p.top_k + threadIdx.x];
+    if (j >= 0 && j < row.V && writes(row, (int)j, chunk, v0, v1)) {
+      float d = p.dtop_logprobs[(int64_t)r * p.top_k + threadIdx.x];
       if (counted && j == t) d += w;
       out[j] = from_f32<T>(fmaf(d, p.inv_temperature, value(to_f32(row.x[j]))));
     }
-  } else if (threadIdx.x == kMaxTop && counted && good && w != 0.f && in_chunk(row, (int)t, chunk)) {
+  } else if (threadIdx.x == kMaxTop && counted && good && w != 0.f && writes(row, (int)t, chunk, v0, v1)) {
     for (int k = 0; k < p.top_k; ++k)
-      if (p.top_ids[r * p.top_k + k] == t) return;
+      if (p.top_ids[(int64_t)r * p.top_k + k] == t) return;
     out[t] = from_f32<T>(fmaf(w, p.inv_temperature, value(to_f32(row.x[t]))));
   }
 }
@@ -690,34 +701,72 @@ struct Teacher {
   bool bad;       // an id out of range
 };
 
-__device__ __forceinline__ float teacher_q(const LogitsArgs& p, int64_t id, float logit, float m, float logs, float& lq) {
+__device__ __forceinline__ float teacher_q(const LogitsArgs& p, int id, float logit, float m, float logs, float& lq) {
   lq = -kInf;
   if (id < 0) return 0.f;
   lq = (logit - m) * p.inv_temperature - logs;
   return expf(lq);
 }
 
-// By one warp.
-__device__ Teacher teacher_stats(const LogitsArgs& p, int64_t r) {
-  const int64_t* ids = p.teacher_ids + r * p.entries;
-  const float* logits = p.teacher_logits + r * p.entries;
-  const int lane = threadIdx.x % 32;
-  float m = -kInf;
-  bool bad = false, some = false;
-  for (int k = lane; k < p.entries; k += 32) {
-    bad |= ids[k] < -1 || ids[k] >= p.vocab;
-    some |= ids[k] >= 0;
-    if (ids[k] >= 0) m = fmaxf(m, logits[k]);
+constexpr int kPerThread = kMaxEntries / kThreads;  // entries of a thread: threadIdx.x + i * kThreads
+
+// A thread's entries of a row, read at the start, while the block has nothing
+// else to do, for the end.
+struct Entries {
+  int id[kPerThread];  // -1: none
+  float logit[kPerThread];
+  bool bad;            // one of them is out of range
+  __device__ Entries(const LogitsArgs& p, uint32_t r) : bad(false) {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const int k = threadIdx.x + i * kThreads;
+      id[i] = -1;
+      logit[i] = 0.f;
+      if (k < p.entries) {
+        const int64_t got = p.teacher_ids[(int64_t)r * p.entries + k];
+        logit[i] = p.teacher_logits[(int64_t)r * p.entries + k];
+        if (got >= 0 && got < p.vocab) id[i] = (int)got;
+        else bad |= got != -1;
+      }
+    }
   }
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+};
+
+__device__ __forceinline__ float sum_block(float v) {
+  __shared__ float part[kWarps];
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
+  __syncthreads();
+  v = part[0];
+#pragma unroll
+  for (int i = 1; i < kWarps; ++i) v += part[i];
+  return v;
+}
+
+// By the whole block.
+__device__ __forceinline__ Teacher teacher_stats(const LogitsArgs& p, uint32_t r, const Entries& e) {
+  __shared__ float part[kWarps];
   Teacher t;
-  t.bad = __any_sync(~0u, bad);
-  some = __any_sync(~0u, some);
+  bool some = false;
+  float m = -kInf;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i)
+    if (e.id[i] >= 0) {
+      some = true;
+      m = fmaxf(m, e.logit[i]);
+    }
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
+  some = __syncthreads_or(some);
+  t.bad = __syncthreads_or(e.bad);
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, part[i]);
   t.m = p.teacher_lse || m == -kInf ? 0.f : m;
   t.logs = p.teacher_lse ? (some ? p.teacher_lse[r] : kInf) : 0.f;
   float s = 0.f, lq;
-  for (int k = lane; k < p.entries; k += 32) s += teacher_q(p, ids[k], logits[k], t.m, t.logs, lq);
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) s += teacher_q(p, e.id[i], e.logit[i], t.m, t.logs, lq);
+  s = sum_block(s);
   if (p.teacher_lse) {
     t.mass = s;
     t.rest = some ? fmaxf(0.f, 1.f - s) : 0.f;
@@ -738,66 +787,66 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   __shared__ uint32_t single_marks;
   __shared__ Sums peers[kMaxCluster];
   griddep_wait();
-  const int64_t r = blockIdx.x / C;
+  const uint32_t r = blockIdx.x / C;
   const int rank = C > 1 ? (int)sm100::cluster_ctarank() : 0;
   if (C > 1) cluster_arrive();
   const Row<T> row(p, r);
   const int per = (row.vectors + C - 1) / C;
   const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
-  const int64_t* ids = p.teacher_ids + r * p.entries;
+  const Entries entries(p, r);
+  float given[kPerThread];  // the model's logits there
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) given[i] = rank == 0 && entries.id[i] >= 0 ? to_f32(row.x[entries.id[i]]) : 0.f;
   if constexpr (REST) {
     for (int i = threadIdx.x; i < (v1 - v0 + 3) / 4; i += kThreads) marks[i] = 0;
     if (threadIdx.x == 0) single_marks = 0;
     __syncthreads();
-    if (threadIdx.x < p.entries) {
-      const int64_t id = ids[threadIdx.x];
-      if (id >= 0 && id < row.V) {
-        const int v = row.place((int)id);
-        if (v < 0) atomicOr(&single_marks, 1u << (-1 - v));
-        else if (v >= v0 && v < v1) atomicOr(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + ((int)id - row.lead) % Row<T>::E));
-      }
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const int id = entries.id[i];
+      if (id < 0) continue;
+      const int v = row.place(id);
+      if (v < 0) atomicOr(&single_marks, 1u << (-1 - v));
+      else if (v >= v0 && v < v1) atomicOr(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + (id - row.lead) % Row<T>::E));
     }
     __syncthreads();
   }
   Running<T, false, REST> run(scale_of(p));
   const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
-  each_vectors(row, v0, v1, [&](const uint4* raw, int v, auto n) {
+  each_vectors(row, v0, v1, [&](const uint4* raw, int v) {
     float top = -kInf;
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (u < n) top = fmaxf(top, Vec<T>::max(raw[u]));
+    for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, Vec<T>::max(raw[u]));
     run.see(top);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u)
-      if (u < n) run.add(raw[u], REST ? mark[v + u * kThreads - v0] : 0);
+    for (int u = 0; u < kUnroll; ++u) run.add(raw[u], REST && v + u * kThreads < v1 ? mark[v + u * kThreads - v0] : 0);
   });
   if (rank == 0 && threadIdx.x < row.singles)
     run.add_single(to_f32(row.x[row.single(threadIdx.x)]), REST && (single_marks >> threadIdx.x & 1));
-  Sums a = block_merge(run.sums(), run.c);
+  Sums a = merge_block<false, REST>(run.sums(), run.c);
   if (C > 1) {
     cluster_wait();
     if (threadIdx.x == 0) *in_block(&peers[rank], 0) = a;
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    a = peers[0];
-    for (int i = 1; i < C; ++i) a = merge(a, peers[i], run.c);
+    a = merge_lanes<false, REST>(peers[threadIdx.x % C], run.c, C);
   }
   const Stats st = finish<T, false, REST>(p, row, a, [&](int j) {
     for (int k = 0; k < p.entries; ++k)
-      if (ids[k] == j) return true;
+      if (p.teacher_ids[(int64_t)r * p.entries + k] == j) return true;
     return false;
   });
-  if (threadIdx.x >= 32) return;
-  const Teacher t = teacher_stats(p, r);
+  const Teacher t = teacher_stats(p, r, entries);
   float loss = 0.f;
-  if (!t.bad)
-    for (int k = threadIdx.x; k < p.entries; k += 32) {
-      float lq;
-      const float q = teacher_q(p, ids[k], p.teacher_logits[r * p.entries + k], t.m, t.logs, lq);
-      if (q != 0.f) loss += q * (lq - st.logprob(to_f32(row.x[ids[k]])));
-    }
-  for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(~0u, loss, o);
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    float lq;
+    const float q = teacher_q(p, entries.id[i], entries.logit[i], t.m, t.logs, lq);
+    if (q != 0.f) loss += q * (lq - st.logprob(given[i]));
+  }
+  __syncthreads();
+  loss = sum_block(loss);
   float ratio = 0.f;  // q_r / p_r
   if (REST && t.rest > 0.f) {
     ratio = t.rest / st.rest;
@@ -810,7 +859,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   }
   p.loss[r] = loss;
   if (p.stats) {
-    float* keep = p.stats + r * kDistillStats;
+    float* keep = p.stats + (int64_t)r * kDistillStats;
     keep[0] = st.m;
     keep[1] = st.l2s;
     keep[2] = t.m;
@@ -821,34 +870,41 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p, int chunks) {
-  __shared__ int id_of[kMaxEntries];
+__global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p, int chunks, int span) {
+  __shared__ __align__(16) int id_of[kMaxEntries];
   __shared__ float q_of[kMaxEntries];
   griddep_wait();
-  const int64_t r = blockIdx.x / chunks;
-  const int chunk = blockIdx.x % chunks;
+  const uint32_t r = blockIdx.x / chunks;
+  const int chunk = blockIdx.x - r * chunks;
   const Row<T> row(p, r);
-  T* out = (T*)p.dlogits + r * p.vocab;
-  const float* keep = p.stats + r * kDistillStats;
+  const int v0 = min(chunk * span, row.vectors), v1 = min(v0 + span, row.vectors);
+  T* out = (T*)p.dlogits + (int64_t)r * p.vocab;
+  const float* keep = p.stats + (int64_t)r * kDistillStats;
   const Stats st = stats_of(p, keep[0], keep[1]);
   const float g = p.dloss[r] * p.inv_temperature;
   // dlogits_j = p_j outer, or for an entry p_j inner - its q
   const float inner = keep[4] * g, outer = (keep[4] - keep[5]) * g;
-  if (threadIdx.x < p.entries) {
-    const int64_t id = p.teacher_ids[r * p.entries + threadIdx.x];
+  const Entries entries(p, r);
+  float given[kPerThread];
+  bool mine[kPerThread];  // this block writes it
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
     float lq;
-    q_of[threadIdx.x] = teacher_q(p, id, p.teacher_logits[r * p.entries + threadIdx.x], keep[2], keep[3], lq);
-    id_of[threadIdx.x] = id >= 0 && id < row.V ? (int)id : -1;
+    const int k = threadIdx.x + i * kThreads;
+    q_of[k] = teacher_q(p, entries.id[i], entries.logit[i], keep[2], keep[3], lq);
+    id_of[k] = entries.id[i];
+    mine[i] = entries.id[i] >= 0 && writes(row, entries.id[i], chunk, v0, v1);
+    given[i] = mine[i] ? to_f32(row.x[entries.id[i]]) : 0.f;
   }
   auto prob = [&](float x) { return exp2_approx(st.y(x) - st.l2s); };
   const bool zero = g == 0.f || (st.empty() && !isnan(inner));
   if (st.far) {
-    const int j0 = row.lead + chunk * kChunk * Row<T>::E, j1 = row.lead + min((chunk + 1) * kChunk, row.vectors) * Row<T>::E;
-    for (int j = j0 + threadIdx.x; j < j1; j += kThreads) out[j] = from_f32<T>(zero ? 0.f : prob(to_f32(row.x[j])) * outer);
+    for (int j = row.lead + v0 * Row<T>::E + threadIdx.x; j < row.lead + v1 * Row<T>::E; j += kThreads)
+      out[j] = from_f32<T>(zero ? 0.f : prob(to_f32(row.x[j])) * outer);
   } else {
     const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
     const uint64_t o2 = sm100::f2_splat(outer);
-    map_chunk(row, out, chunk, zero, [&](const uint4& raw, int i) {
+    map_vectors(row, out, v0, v1, zero, [&](const uint4& raw, int i) {
       const float2 f = sm100::f2_split(sm100::f2_add(sm100::f2_fma(Vec<T>::pair(raw, i), c2, nM), nl));
       return sm100::f2_mul(sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y))), o2);
     });
@@ -859,28 +915,39 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   }
   if (zero) return;
   __syncthreads();
-  // the entries once more, each by the first that names it
-  if (threadIdx.x >= p.entries) return;
-  const int j = id_of[threadIdx.x];
-  if (j < 0 || !in_chunk(row, j, chunk)) return;
-  float q = 0.f;
-  for (int k = 0; k < p.entries; ++k)
-    if (id_of[k] == j) {
-      if (k < threadIdx.x) return;
+  // the entries once more, each by the first that names it, with the q of all that do
+  const int4* four = reinterpret_cast<const int4*>(id_of);
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) {
+    if (!mine[i]) continue;
+    const int j = entries.id[i], self = threadIdx.x + i * kThreads;
+    float q = 0.f;
+    int first = self;
+    auto same = [&](int k) {
+      first = min(first, k);
       q += q_of[k];
+    };
+    for (int k = 0; 4 * k < p.entries; ++k) {
+      const int4 ids = four[k];
+      if (ids.x == j) same(4 * k);
+      if (ids.y == j) same(4 * k + 1);
+      if (ids.z == j) same(4 * k + 2);
+      if (ids.w == j) same(4 * k + 3);
     }
-  out[j] = from_f32<T>(prob(to_f32(row.x[j])) * inner - q * g);
+    if (first == self) out[j] = from_f32<T>(prob(given[i]) * inner - q * g);
+  }
 }
 
 // ---------------------------------------------------------------------------
 // Launches
 // ---------------------------------------------------------------------------
-// Blocks of a cluster, which share a row: as many as give every SM two blocks,
-// while each keeps a full round of loads, and as a block's shared memory asks
-// for (`bytes` per vector).
+// Blocks of a cluster, which share a row: as many as give every SM kBlocks,
+// while a thread keeps a vector or two, and as a block's shared memory asks for
+// (`bytes` per vector).
+constexpr int kBlocks = 6;
 int cluster_size(int64_t rows, int64_t vectors, int bytes) {
   int c = 1;
-  while (c < kMaxCluster && ((rows * c < 2 * fakla_sm_count() && vectors / (2 * c) >= kThreads) ||
+  while (c < kMaxCluster && ((rows * c < kBlocks * fakla_sm_count() && vectors / (2 * c) >= kThreads) ||
                              vectors / c * bytes > (48 << 10)))
     c *= 2;
   return c;
@@ -898,11 +965,16 @@ cudaError_t launch_rows(K kernel, const LogitsArgs& p, int per_vector, int bytes
   return launch_chained(kernel, dim3((unsigned)(p.batch * p.rows * c)), dim3(kThreads), smem, stream, (unsigned)c, p, c);
 }
 
+// A row's gradient is split into spans of whole rounds of loads, as long as
+// every SM still gets kBlocks blocks.
 template <typename K>
-cudaError_t launch_chunks(K kernel, const LogitsArgs& p, int per_vector, cudaStream_t stream) {
-  const int chunks = (int)((p.vocab / per_vector + kChunk - 1) / kChunk);
-  const int n = chunks > 0 ? chunks : 1;
-  return launch_chained(kernel, dim3((unsigned)(p.batch * p.rows * n)), dim3(kThreads), 0, stream, 1u, p, n);
+cudaError_t launch_spans(K kernel, const LogitsArgs& p, int per_vector, cudaStream_t stream) {
+  const int64_t rows = p.batch * p.rows, rounds = (p.vocab / per_vector + kRound - 1) / kRound;
+  int64_t chunks = (kBlocks * fakla_sm_count() + rows - 1) / rows;
+  if (chunks > rounds) chunks = rounds;
+  if (chunks < 1) chunks = 1;
+  const int span = (int)((rounds + chunks - 1) / chunks) * kRound;
+  return launch_chained(kernel, dim3((unsigned)(rows * chunks)), dim3(kThreads), 0, stream, 1u, p, (int)chunks, span);
 }
 
 template <typename F>
@@ -922,7 +994,7 @@ cudaError_t launch_token_logprobs(int dtype, const LogitsArgs& p, cudaStream_t s
 
 cudaError_t launch_token_logprobs_backward(int dtype, const LogitsArgs& p, cudaStream_t stream) {
   return by_type(dtype, [&](auto t) {
-    return launch_chunks(token_logprobs_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
+    return launch_spans(token_logprobs_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
   });
 }
 
@@ -936,7 +1008,7 @@ cudaError_t launch_distill(int dtype, const LogitsArgs& p, cudaStream_t stream) 
 
 cudaError_t launch_distill_backward(int dtype, const LogitsArgs& p, cudaStream_t stream) {
   return by_type(dtype, [&](auto t) {
-    return launch_chunks(distill_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
+    return launch_spans(distill_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
   });
 }
 
