@@ -47,6 +47,19 @@ def _stream(dev: torch.device) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
+def _launch(dev: torch.device, fn, *args) -> None:
+    """fn(*args, current stream of dev) with dev current; raises on an error
+    status. Leaves the device alone where it is current already: entering and
+    leaving torch.cuda.device costs as much as a small launch."""
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if rc:
+        _lib.check(rc)
+
+
 def _require(cond: bool, msg: str) -> None:
     if not cond:
         raise RuntimeError(msg)

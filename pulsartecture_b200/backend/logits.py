@@ -13,10 +13,11 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .interface import _check_device, _dtype_code, _needs_grad, _ptr, _require, _stream
+from .interface import _launch, _ptr
 
 MAX_TOP_K = 32
 MAX_ENTRIES = 256
+_DTYPES = {torch.float32: _lib.FAKLA_F32, torch.bfloat16: _lib.FAKLA_BF16}
 
 
 class TokenLogprobs(NamedTuple):
@@ -26,45 +27,50 @@ class TokenLogprobs(NamedTuple):
     top_ids: Optional[torch.Tensor]        # (..., top_k) int64, or None
 
 
-def _as_rows(logits: torch.Tensor) -> torch.Tensor:
-    """(batch, rows, vocab) over the same values: a view wherever the leading
-    dimensions come down to two strides (a slice of positions or a padded
-    vocabulary does), a dense copy otherwise."""
-    if logits.stride(-1) != 1 and logits.shape[-1] != 1:
+def _as_rows(logits: torch.Tensor):
+    """logits, and how its rows lie: (batch, rows, vocab, batch stride, row
+    stride). A view wherever the leading dimensions come down to two strides (a
+    slice of positions or of a padded vocabulary does), a dense copy otherwise."""
+    nd = logits.dim()
+    if nd > 3:
+        logits = logits.reshape(-1, *logits.shape[-2:])
+        nd = 3
+    st = logits.stride()
+    if st[-1] != 1 and logits.shape[-1] != 1:
         logits = logits.contiguous()
-    if logits.dim() == 3:
-        return logits
-    if logits.dim() < 3:
-        return logits.reshape(1, -1, logits.shape[-1])
-    return logits.reshape(-1, *logits.shape[-2:])
+        st = logits.stride()
+    if nd == 3:
+        return logits, (*logits.shape, st[0], st[1])
+    if nd == 2:
+        return logits, (1, *logits.shape, 0, st[0])
+    return logits, (1, 1, *logits.shape, 0, 0)
 
 
-def _check_rows(logits: torch.Tensor, given, names, lead_of) -> torch.device:
-    _require(logits.dim() >= 1 and logits.shape[-1] >= 1, "logits must be (..., vocab)")
-    dev = _check_device([logits, *given], ["logits", *names])
-    lead = tuple(logits.shape[:-1])
-    for t, n in zip(given, names):
-        if t is not None:
-            got = tuple(t.shape[:len(lead)]) if n in lead_of else tuple(t.shape)
-            _require(got == lead, f"{n} {tuple(t.shape)} does not go with logits {tuple(logits.shape)}")
-    return dev
-
-
-def _check_temperature(temperature: float) -> float:
+def _check_rows(logits: torch.Tensor, temperature: float):
+    """Returns the leading shape, the dtype code and the temperature."""
     temperature = float(temperature)
-    _require(1e-30 <= temperature <= 1e30, f"temperature must be positive (1e-30 to 1e30), got {temperature}")
-    return temperature
+    if not 1e-30 <= temperature <= 1e30:
+        raise RuntimeError(f"temperature must be positive (1e-30 to 1e30), got {temperature}")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise RuntimeError("logits must be (..., vocab)")
+    code = _DTYPES.get(logits.dtype)
+    if code is None:
+        raise RuntimeError(f"logits must be float32 or bfloat16, got {logits.dtype}")
+    if not logits.is_cuda:
+        raise RuntimeError("logits must be a CUDA tensor (libfakla has no CPU path)")
+    return logits.shape[:-1], code, temperature
 
 
 class _TokenLogprobsFn(torch.autograd.Function):
     """fakla_token_logprobs with gradients (fakla_token_logprobs_backward)."""
 
     @staticmethod
-    def forward(ctx, logits, targets, top_k, temperature, ignore_index):
+    def forward(ctx, logits, targets, top_k, temperature, ignore_index, code):
         ctx.set_materialize_grads(False)
-        lp, ent, top, ids, stats = _run_logprobs(logits, targets, top_k, temperature, ignore_index, True)
-        ctx.save_for_backward(logits, targets, stats, ent, ids)
-        ctx.top_k, ctx.temperature, ctx.ignore_index = top_k, temperature, ignore_index
+        rows, at = _as_rows(logits)
+        lp, ent, top, ids, stats = _run_logprobs(rows, at, targets, top_k, temperature, ignore_index, code, True)
+        ctx.save_for_backward(rows, targets, stats, ent, ids)
+        ctx.form = at, top_k, temperature, ignore_index, code, logits.shape
         if top_k:
             ctx.mark_non_differentiable(ids)
         return lp, ent, top, ids
@@ -72,31 +78,24 @@ class _TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dlp, dent, dtop, _):
-        logits, targets, stats, ent, ids = ctx.saved_tensors
-        dlp, dent, dtop = (None if t is None else t.contiguous().float() for t in (dlp, dent, dtop))
-        dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        dev = logits.device
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().fakla_token_logprobs_backward(
-                _ptr(logits), _ptr(targets), _ptr(stats), _ptr(ent), _ptr(ids), _ptr(dlp), _ptr(dent), _ptr(dtop),
-                _ptr(dlogits), *logits.shape, logits.stride(0), logits.stride(1), ctx.top_k, ctx.temperature,
-                ctx.ignore_index, _dtype_code(logits), _stream(dev)))
-        return dlogits, None, None, None, None
+        rows, targets, stats, ent, ids = ctx.saved_tensors
+        at, top_k, temperature, ignore_index, code, shape = ctx.form
+        dlp, dent, dtop = (None if t is None else t.contiguous() for t in (dlp, dent, dtop))
+        dlogits = torch.empty(shape, device=rows.device, dtype=rows.dtype)
+        _launch(rows.device, _lib.lib().fakla_token_logprobs_backward, _ptr(rows), _ptr(targets), _ptr(stats), _ptr(ent),
+                _ptr(ids), _ptr(dlp), _ptr(dent), _ptr(dtop), _ptr(dlogits), *at, top_k, temperature, ignore_index, code)
+        return dlogits, None, None, None, None, None
 
 
-def _run_logprobs(logits, targets, top_k, temperature, ignore_index, save):
-    """logits (batch, rows, vocab); everything it returns is (batch, rows, ...)."""
-    dev = logits.device
-    lead = logits.shape[:2]
+def _run_logprobs(rows, at, targets, top_k, temperature, ignore_index, code, save):
+    dev, lead = rows.device, targets.shape
     lp = torch.empty(lead, device=dev, dtype=torch.float32)
     ent = torch.empty(lead, device=dev, dtype=torch.float32)
-    top = torch.empty(*lead, top_k, device=dev, dtype=torch.float32) if top_k else None
-    ids = torch.empty(*lead, top_k, device=dev, dtype=torch.int64) if top_k else None
-    stats = torch.empty(*lead, 2, device=dev, dtype=torch.float32) if save else None
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().fakla_token_logprobs(
-            _ptr(logits), _ptr(targets), _ptr(lp), _ptr(ent), _ptr(top), _ptr(ids), _ptr(stats), *logits.shape,
-            logits.stride(0), logits.stride(1), top_k, temperature, ignore_index, _dtype_code(logits), _stream(dev)))
+    top = torch.empty((*lead, top_k), device=dev, dtype=torch.float32) if top_k else None
+    ids = torch.empty((*lead, top_k), device=dev, dtype=torch.int64) if top_k else None
+    stats = torch.empty((at[0] * at[1], 2), device=dev, dtype=torch.float32) if save else None
+    _launch(dev, _lib.lib().fakla_token_logprobs, _ptr(rows), _ptr(targets), _ptr(lp), _ptr(ent), _ptr(top), _ptr(ids),
+            _ptr(stats), *at, top_k, temperature, ignore_index, code)
     return lp, ent, top, ids, stats
 
 
@@ -121,63 +120,57 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
     tokens, put ignore_index at the last position's target rather than slicing
     the logits: a slice's gradient is copied once more by autograd.
     """
-    temperature = _check_temperature(temperature)
-    _check_rows(logits, [targets], ["targets"], ())
-    _require(targets.dtype == torch.int64, "targets must be int64")
-    V = logits.shape[-1]
-    _require(0 <= top_k <= min(MAX_TOP_K, V), f"top_k must be in [0, min({MAX_TOP_K}, vocab)], got {top_k}")
-    _dtype_code(logits)
-    lead = logits.shape[:-1]
+    lead, code, temperature = _check_rows(logits, temperature)
+    if targets.shape != lead:
+        raise RuntimeError(f"targets {tuple(targets.shape)} do not go with logits {tuple(logits.shape)}")
+    if targets.dtype != torch.int64:
+        raise RuntimeError("targets must be int64")
+    if targets.device != logits.device:
+        raise RuntimeError(f"targets are on {targets.device}, expected {logits.device}")
+    if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
+        raise RuntimeError(f"top_k must be in [0, min({MAX_TOP_K}, vocab)], got {top_k}")
     if targets.numel() == 0:
         empty = logits.new_empty(lead, dtype=torch.float32) + 0 * logits.sum()
         top = ids = None
         if top_k:
             top, ids = logits.new_empty(*lead, top_k, dtype=torch.float32), targets.new_empty(*lead, top_k)
         return TokenLogprobs(empty, empty.clone(), top, ids)
-    rows = _as_rows(logits)
-    flat = targets.contiguous()
-    if _needs_grad(logits):
-        lp, ent, top, ids = _TokenLogprobsFn.apply(rows, flat, top_k, temperature, ignore_index)
-    else:
-        lp, ent, top, ids, _ = _run_logprobs(rows, flat, top_k, temperature, ignore_index, False)
-    if top_k:
-        top, ids = top.reshape(*lead, top_k), ids.reshape(*lead, top_k)
-    return TokenLogprobs(lp.reshape(lead), ent.reshape(lead), top, ids)
+    targets = targets.contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobsFn.apply(logits, targets, top_k, temperature, ignore_index, code))
+    rows, at = _as_rows(logits)
+    return TokenLogprobs(*_run_logprobs(rows, at, targets, top_k, temperature, ignore_index, code, False)[:4])
 
 
 class _DistillFn(torch.autograd.Function):
     """fakla_distill_topk with gradients (fakla_distill_topk_backward)."""
 
     @staticmethod
-    def forward(ctx, logits, ids, teacher, lse, temperature):
-        loss, stats = _run_distill(logits, ids, teacher, lse, temperature, True)
-        ctx.save_for_backward(logits, ids, teacher, lse, stats)
-        ctx.temperature = temperature
+    def forward(ctx, logits, ids, teacher, lse, temperature, code):
+        rows, at = _as_rows(logits)
+        loss, stats = _run_distill(rows, at, ids, teacher, lse, temperature, code, True)
+        ctx.save_for_backward(rows, ids, teacher, lse, stats)
+        ctx.form = at, temperature, code, logits.shape
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss):
-        logits, ids, teacher, lse, stats = ctx.saved_tensors
-        dloss = dloss.contiguous().float()
-        dlogits = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        dev = logits.device
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().fakla_distill_topk_backward(
-                _ptr(logits), _ptr(ids), _ptr(teacher), _ptr(lse), _ptr(stats), _ptr(dloss), _ptr(dlogits),
-                *logits.shape, logits.stride(0), logits.stride(1), ids.shape[-1], ctx.temperature,
-                _dtype_code(logits), _stream(dev)))
-        return dlogits, None, None, None, None
+        rows, ids, teacher, lse, stats = ctx.saved_tensors
+        at, temperature, code, shape = ctx.form
+        dloss = dloss.contiguous()
+        dlogits = torch.empty(shape, device=rows.device, dtype=rows.dtype)
+        _launch(rows.device, _lib.lib().fakla_distill_topk_backward, _ptr(rows), _ptr(ids), _ptr(teacher), _ptr(lse),
+                _ptr(stats), _ptr(dloss), _ptr(dlogits), *at, ids.shape[-1], temperature, code)
+        return dlogits, None, None, None, None, None
 
 
-def _run_distill(logits, ids, teacher, lse, temperature, save):
-    dev = logits.device
-    loss = torch.empty(logits.shape[:2], device=dev, dtype=torch.float32)
-    stats = torch.empty(*logits.shape[:2], 8, device=dev, dtype=torch.float32) if save else None
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().fakla_distill_topk(
-            _ptr(logits), _ptr(ids), _ptr(teacher), _ptr(lse), _ptr(loss), _ptr(stats), *logits.shape,
-            logits.stride(0), logits.stride(1), ids.shape[-1], temperature, _dtype_code(logits), _stream(dev)))
+def _run_distill(rows, at, ids, teacher, lse, temperature, code, save):
+    dev = rows.device
+    loss = torch.empty(ids.shape[:-1], device=dev, dtype=torch.float32)
+    stats = torch.empty((at[0] * at[1], 8), device=dev, dtype=torch.float32) if save else None
+    _launch(dev, _lib.lib().fakla_distill_topk, _ptr(rows), _ptr(ids), _ptr(teacher), _ptr(lse), _ptr(loss), _ptr(stats),
+            *at, ids.shape[-1], temperature, code)
     return loss, stats
 
 
@@ -200,26 +193,28 @@ def distill_topk(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     Differentiable in logits; the teacher's side gets no gradient. The loss is
     not multiplied by temperature squared.
     """
-    temperature = _check_temperature(temperature)
-    _check_rows(logits, [teacher_ids, teacher_logits, teacher_lse], ["teacher_ids", "teacher_logits", "teacher_lse"],
-                ("teacher_ids", "teacher_logits"))
-    lead = logits.shape[:-1]
-    _require(teacher_ids.dim() == logits.dim() and teacher_ids.shape == teacher_logits.shape,
-             "teacher_ids and teacher_logits must both be (..., K)")
-    _require(teacher_ids.dtype == torch.int64, "teacher_ids must be int64")
-    _require(teacher_logits.is_floating_point() and (teacher_lse is None or teacher_lse.is_floating_point()),
-             "teacher_logits and teacher_lse must be floating")
+    lead, code, temperature = _check_rows(logits, temperature)
+    if teacher_ids.dim() != logits.dim() or teacher_ids.shape != teacher_logits.shape or teacher_ids.shape[:-1] != lead:
+        raise RuntimeError(f"teacher_ids {tuple(teacher_ids.shape)} and teacher_logits {tuple(teacher_logits.shape)} "
+                           f"must both be (..., K) for logits {tuple(logits.shape)}")
+    if teacher_lse is not None and teacher_lse.shape != lead:
+        raise RuntimeError(f"teacher_lse {tuple(teacher_lse.shape)} does not go with logits {tuple(logits.shape)}")
+    if teacher_ids.dtype != torch.int64:
+        raise RuntimeError("teacher_ids must be int64")
+    if not teacher_logits.is_floating_point() or (teacher_lse is not None and not teacher_lse.is_floating_point()):
+        raise RuntimeError("teacher_logits and teacher_lse must be floating")
+    dev = logits.device
+    if teacher_ids.device != dev or teacher_logits.device != dev or (teacher_lse is not None and teacher_lse.device != dev):
+        raise RuntimeError(f"the teacher's tensors must be on the device of logits ({dev})")
     K = teacher_ids.shape[-1]
-    _require(1 <= K <= MAX_ENTRIES, f"K must be in [1, {MAX_ENTRIES}], got {K}")
-    _dtype_code(logits)
+    if not 1 <= K <= MAX_ENTRIES:
+        raise RuntimeError(f"K must be in [1, {MAX_ENTRIES}], got {K}")
     if teacher_ids.numel() == 0:
         return logits.new_empty(lead, dtype=torch.float32) + 0 * logits.sum()
-    rows = _as_rows(logits)
     ids = teacher_ids.contiguous()
-    teacher = teacher_logits.detach().float().contiguous()
-    lse = None if teacher_lse is None else teacher_lse.detach().float().contiguous()
-    if _needs_grad(logits):
-        loss = _DistillFn.apply(rows, ids, teacher, lse, temperature)
-    else:
-        loss, _ = _run_distill(rows, ids, teacher, lse, temperature, False)
-    return loss.reshape(lead)
+    teacher = teacher_logits.detach().to(torch.float32).contiguous()
+    lse = None if teacher_lse is None else teacher_lse.detach().to(torch.float32).contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _DistillFn.apply(logits, ids, teacher, lse, temperature, code)
+    rows, at = _as_rows(logits)
+    return _run_distill(rows, at, ids, teacher, lse, temperature, code, False)[0]

@@ -15,24 +15,38 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .interface import _check_device, _dtype_code, _needs_grad, _ptr, _require, _stream
+from .interface import _launch, _ptr
 
 GATE_ACTIVATIONS = {"sigmoid": _lib.FAKLA_ACT_SIGMOID, "identity": _lib.FAKLA_ACT_IDENTITY}
+_DTYPES = {torch.float32: _lib.FAKLA_F32, torch.bfloat16: _lib.FAKLA_BF16}
 
 
 def _check_gated(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor], gate_act: str, ndim: int):
-    """Checks shared by the scan and the step: the device and the dtype code."""
-    shape = "(B, T, D)" if ndim == 3 else "(N, D)"
-    _require(x.dim() == ndim and gate.dim() == ndim, f"x and gate must be {shape}")
-    _require(x.shape == gate.shape, f"x {tuple(x.shape)} and gate {tuple(gate.shape)} shapes must match")
-    _require(x.dtype == gate.dtype, "x and gate must have the same dtype")
-    _require(gate_act in GATE_ACTIVATIONS, f"unknown gate_act {gate_act!r}; choose from {sorted(GATE_ACTIVATIONS)}")
-    dev = _check_device([x, gate, state], ["x", "gate", "state"])
+    """Checks shared by the scan and the step; returns the device, the dtype
+    code and the gate activation's."""
+    if x.dim() != ndim or gate.dim() != ndim:
+        raise RuntimeError(f"x and gate must be {'(B, T, D)' if ndim == 3 else '(N, D)'}")
+    if x.shape != gate.shape:
+        raise RuntimeError(f"x {tuple(x.shape)} and gate {tuple(gate.shape)} shapes must match")
+    if x.dtype != gate.dtype:
+        raise RuntimeError("x and gate must have the same dtype")
+    act = GATE_ACTIVATIONS.get(gate_act)
+    if act is None:
+        raise RuntimeError(f"unknown gate_act {gate_act!r}; choose from {sorted(GATE_ACTIVATIONS)}")
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        raise RuntimeError(f"gated_scan supports float32 and bfloat16 inputs, got {x.dtype}")
+    dev = x.device
+    if dev.type != "cuda":
+        raise RuntimeError("x must be a CUDA tensor (libfakla has no CPU path)")
+    if gate.device != dev or (state is not None and state.device != dev):
+        raise RuntimeError(f"x, gate and state must be on one device ({dev})")
     if state is not None:
-        expected = (x.shape[0], x.shape[-1])
-        _require(tuple(state.shape) == expected, f"state must be {expected}, got {tuple(state.shape)}")
-        _require(state.dtype == torch.float32, "state must be float32")
-    return dev, _dtype_code(x)
+        if state.dim() != 2 or state.shape[0] != x.shape[0] or state.shape[1] != x.shape[-1]:
+            raise RuntimeError(f"state must be {(x.shape[0], x.shape[-1])}, got {tuple(state.shape)}")
+        if state.dtype != torch.float32:
+            raise RuntimeError("state must be float32")
+    return dev, code, act
 
 
 def _dense_channels(t: torch.Tensor) -> torch.Tensor:
@@ -44,45 +58,43 @@ class _GatedScanFn(torch.autograd.Function):
     """fakla_gated_scan with gradients (fakla_gated_scan_backward)."""
 
     @staticmethod
-    def forward(ctx, x, gate, state, act, mix):
+    def forward(ctx, x, gate, state, act, mix, code):
         ctx.set_materialize_grads(False)
-        out, final, saved = _run_scan(x, gate, state, act, mix, True, True)
+        out, final, saved = _run_scan(x, gate, state, act, mix, code, True, True)
         ctx.save_for_backward(x, gate, saved)
-        ctx.act, ctx.mix, ctx.has_state = act, mix, state is not None
+        ctx.form = act, mix, code, state is not None
         return out, final
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, dfinal):
         x, gate, saved = ctx.saved_tensors
+        act, mix, code, has_state = ctx.form
         B, T, D = x.shape
         dev = x.device
-        dout = torch.zeros(B, T, D, device=dev, dtype=x.dtype) if dout is None else dout.contiguous().to(dtype=x.dtype)
-        dfinal = None if dfinal is None else dfinal.contiguous().float()
-        dx = torch.empty(B, T, D, device=dev, dtype=x.dtype)
-        dgate = torch.empty_like(dx)
-        dstate = torch.empty(B, D, device=dev, dtype=torch.float32) if ctx.has_state else None
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().fakla_gated_scan_backward(
-                _ptr(x), _ptr(gate), _ptr(saved), _ptr(dout), _ptr(dfinal), _ptr(dx), _ptr(dgate), _ptr(dstate),
-                B, T, D, x.stride(0), x.stride(1), gate.stride(0), gate.stride(1), ctx.act, ctx.mix,
-                _dtype_code(x), _stream(dev)))
-        return dx, dgate, dstate, None, None
+        dx = torch.empty((B, T, D), device=dev, dtype=x.dtype)
+        dgate = torch.empty((B, T, D), device=dev, dtype=x.dtype)
+        dstate = torch.empty((B, D), device=dev, dtype=torch.float32) if has_state else None
+        dout = torch.zeros_like(dx) if dout is None else dout.contiguous()
+        dfinal = None if dfinal is None else dfinal.contiguous()
+        xb, xt, _ = x.stride()
+        gb, gt, _ = gate.stride()
+        _launch(dev, _lib.lib().fakla_gated_scan_backward, _ptr(x), _ptr(gate), _ptr(saved), _ptr(dout), _ptr(dfinal),
+                _ptr(dx), _ptr(dgate), _ptr(dstate), B, T, D, xb, xt, gb, gt, act, mix, code)
+        return dx, dgate, dstate, None, None, None
 
 
-def _run_scan(x, gate, state, act, mix, return_state, save):
+def _run_scan(x, gate, state, act, mix, code, return_state, save):
     B, T, D = x.shape
     dev = x.device
-    out = torch.empty(B, T, D, device=dev, dtype=x.dtype)
-    final = torch.empty(B, D, device=dev, dtype=torch.float32) if return_state else None
     L = _lib.lib()
-    saved = None
-    if save:
-        saved = torch.empty(L.fakla_gated_scan_saved_bytes(B, T, D), device=dev, dtype=torch.uint8)
-    with torch.cuda.device(dev):
-        _lib.check(L.fakla_gated_scan(
-            _ptr(x), _ptr(gate), _ptr(out), _ptr(state), _ptr(final), _ptr(saved), B, T, D,
-            x.stride(0), x.stride(1), gate.stride(0), gate.stride(1), act, mix, _dtype_code(x), _stream(dev)))
+    out = torch.empty((B, T, D), device=dev, dtype=x.dtype)
+    final = torch.empty((B, D), device=dev, dtype=torch.float32) if return_state else None
+    saved = torch.empty(L.fakla_gated_scan_saved_bytes(B, T, D), device=dev, dtype=torch.uint8) if save else None
+    xb, xt, _ = x.stride()
+    gb, gt, _ = gate.stride()
+    _launch(dev, L.fakla_gated_scan, _ptr(x), _ptr(gate), _ptr(out), _ptr(state), _ptr(final), _ptr(saved), B, T, D,
+            xb, xt, gb, gt, act, mix, code)
     return out, final, saved
 
 
@@ -103,20 +115,21 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor
     A gate of -inf ("sigmoid") or 0 ("identity") forgets the state, so packed
     documents are separated by setting it at their first tokens.
     """
-    dev, _ = _check_gated(x, gate, state, gate_act, 3)
-    B, T, D = x.shape
-    act, mix = GATE_ACTIVATIONS[gate_act], bool(mix)
-    if B * T * D == 0:
+    dev, code, act = _check_gated(x, gate, state, gate_act, 3)
+    mix = bool(mix)
+    if x.numel() == 0:
+        B, T, D = x.shape
         final = None
         if return_state:
             final = state.clone() if state is not None else torch.zeros(B, D, device=dev, dtype=torch.float32)
         return torch.empty(B, T, D, device=dev, dtype=x.dtype), final
     x, gate = _dense_channels(x), _dense_channels(gate)
     state = None if state is None else state.contiguous()
-    if _needs_grad(x, gate, state):
-        out, final = _GatedScanFn.apply(x, gate, state, act, mix)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or
+                                    (state is not None and state.requires_grad)):
+        out, final = _GatedScanFn.apply(x, gate, state, act, mix, code)
         return out, (final if return_state else None)
-    out, final, _ = _run_scan(x, gate, state, act, mix, return_state, False)
+    out, final, _ = _run_scan(x, gate, state, act, mix, code, return_state, False)
     return out, final
 
 
@@ -128,20 +141,21 @@ def gated_scan_step(x: torch.Tensor, gate: torch.Tensor, state: torch.Tensor, *,
     place, or with ``new_state`` (float32, (N, D), contiguous, not overlapping
     it) left as it is and the new one written there. Not differentiable.
     """
-    _require(state is not None, "state is required")
-    dev, code = _check_gated(x, gate, state, gate_act, 2)
-    _require(not _needs_grad(x, gate, state, new_state), "gated_scan_step has no backward; use gated_scan, or torch.no_grad()")
+    if state is None:
+        raise RuntimeError("state is required")
+    dev, code, act = _check_gated(x, gate, state, gate_act, 2)
     target = state if new_state is None else new_state
-    _require(target.device == dev and target.shape == state.shape and target.dtype == torch.float32,
-             "new_state must be a float32 tensor like state, on the same device")
-    _require(state.is_contiguous() and target.is_contiguous(), "state and new_state must be contiguous")
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or state.requires_grad or target.requires_grad):
+        raise RuntimeError("gated_scan_step has no backward; use gated_scan, or torch.no_grad()")
+    if target is not state and (target.device != dev or target.shape != state.shape or target.dtype != torch.float32):
+        raise RuntimeError("new_state must be a float32 tensor like state, on the same device")
+    if not (state.is_contiguous() and target.is_contiguous()):
+        raise RuntimeError("state and new_state must be contiguous")
     N, D = x.shape
-    out = torch.empty(N, D, device=dev, dtype=x.dtype)
+    out = torch.empty((N, D), device=dev, dtype=x.dtype)
     if N * D == 0:
         return out, target
     x, gate = _dense_channels(x), _dense_channels(gate)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().fakla_gated_scan_step(
-            _ptr(x), _ptr(gate), _ptr(out), _ptr(state), _ptr(target), N, D, x.stride(0), gate.stride(0),
-            GATE_ACTIVATIONS[gate_act], bool(mix), code, _stream(dev)))
+    _launch(dev, _lib.lib().fakla_gated_scan_step, _ptr(x), _ptr(gate), _ptr(out), _ptr(state), _ptr(target), N, D,
+            x.stride(0), gate.stride(0), act, bool(mix), code)
     return out, target
