@@ -41,7 +41,7 @@ constexpr int kUnroll = 4;      // 16-byte loads of a thread in flight
 constexpr int kMaxCluster = 8;  // the largest portable cluster
 constexpr int kMaxTop = 32;     // as fakla_token_logprobs takes; also the lanes of a warp
 constexpr int kMaxEntries = 256;  // as fakla_distill_topk takes
-constexpr int kCandidates = 1024;
+constexpr int kCandidates = 512;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kNaN = __builtin_nanf("");
 constexpr float kLog2e = 1.44269504f;
@@ -368,15 +368,14 @@ __device__ __forceinline__ float key_value(uint64_t k) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-// The largest value's key in each thread's vectors is known after the pass
-// that sums them. The k-th largest of 32 such keys, each the largest over one
-// lane of all warps, has k values at or above it, so only values from there up
-// can be among the k largest: some 5 for k = 5 and 130 for k = 32 in a random
-// row. They are in the vectors whose maximum, kept in shared memory from the
-// pass, reaches it; those are listed first and then read again all at once, by
-// a thread per value. Keys differ even between equal values, so rows of ties
-// fill no list: lanes interleave finely, and a row of one value lists its first
-// 256 at most.
+// The pass that sums a row leaves the maximum of each vector in shared memory.
+// Of the 32 lanes, each with the largest maximum that it has in any warp, the
+// k-th largest has k values at or above it, so only values from there up can be
+// among the k largest: some 5 for k = 5 and 130 for k = 32 in a random row. They
+// are in the vectors whose maximum reaches it; those are listed first and then
+// read again all at once, by a thread per value. Keys, which hold the index too,
+// differ even between equal values, so rows of ties fill no list: lanes
+// interleave finely, and a row of one value lists its first 256 or so.
 struct TopSpace {
   uint64_t best[kWarps][32];
   uint64_t list[kCandidates];
@@ -390,14 +389,14 @@ struct TopSpace {
 // their number, more than kCandidates if that or their vectors are too many.
 template <typename T>
 __device__ __forceinline__ int collect(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles,
-                                       const float* most) {
+                                       const T* most) {
   constexpr int E = Row<T>::E;
   const uint64_t floor = sp.floor;
   const float least = floor == 0 ? -kInf : key_value(floor);
   // equal maxima count up to the vector of the floor's own index
   const int last = floor == 0 ? v1 : (key_index(floor) - row.lead) / E;
   for (int v = v0 + threadIdx.x; v < v1; v += kThreads)
-    if (most[v - v0] > least || (most[v - v0] == least && v <= last)) {
+    if (const float m = to_f32(most[v - v0]); m > least || (m == least && v <= last)) {
       const int at = atomicAdd(&sp.vector_count, 1);
       if (at < kCandidates) sp.vectors[at] = v;
     }
@@ -431,22 +430,43 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, ui
   __syncthreads();
 }
 
-// The k largest keys of the block's part of the row, into sp.top. best: the
-// thread's vector with the largest maximum, at: its number (-1: none).
+// The k largest of C blocks' top keys, each in descending order (kMaxTop
+// apart), into top: a key's rank is its place in its own list and the number of
+// larger ones in each other, found by halving.
+__device__ __forceinline__ void merge_lists(const uint64_t* lists, int C, int k, uint64_t* top) {
+  for (int i = threadIdx.x; i < C * k; i += kThreads) {
+    const int own = i / k;
+    const uint64_t key = lists[own * kMaxTop + (i - own * k)];
+    int above = 0;
+    for (int c = 0; c < C; ++c) {
+      const uint64_t* list = lists + c * kMaxTop;
+      int larger = 0;
+#pragma unroll
+      for (int step = kMaxTop / 2; step > 0; step /= 2)
+        if (list[larger + step - 1] > key) larger += step;
+      larger += list[larger] > key;
+      above += larger;
+    }
+    if (above < k) top[above] = key;
+  }
+  __syncthreads();
+}
+
+// The k largest keys of the block's part of the row, into sp.top.
 template <typename T>
 __device__ __forceinline__ void block_top(TopSpace& sp, const Row<T>& row, int v0, int v1, bool singles,
-                                          const float* most, int k, const uint4& best, int at) {
-  uint64_t key = 0;
-  if (at >= 0) {
-    const float m = Vec<T>::max(best);
-#pragma unroll
-    for (int i = Row<T>::E / 2 - 1; i >= 0; --i) {
-      const float2 f = sm100::f2_split(Vec<T>::pair(best, i));
-      const int j = row.lead + at * Row<T>::E + 2 * i;
-      if (f.y == m) key = order_key(f.y, j + 1);
-      if (f.x == m) key = order_key(f.x, j);
+                                          const T* most, int k) {
+  // the thread's largest maximum of a vector, with the last index it can have
+  float best = -kInf;
+  int at = -1;
+  for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
+    const float m = to_f32(most[v - v0]);
+    if (m > best || at < 0) {
+      best = m;
+      at = v;
     }
   }
+  uint64_t key = at < 0 ? 0 : order_key(best, row.lead + at * Row<T>::E + Row<T>::E - 1);
   sp.best[threadIdx.x / 32][threadIdx.x % 32] = key;
   if (threadIdx.x == 0) sp.count = sp.vector_count = 0;
   __syncthreads();
@@ -504,7 +524,8 @@ __device__ __forceinline__ void block_top(TopSpace& sp, const Row<T>& row, int v
 // ---------------------------------------------------------------------------
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, int C) {
-  extern __shared__ float most[];  // TOP: the maximum of each of the block's vectors
+  extern __shared__ __align__(16) unsigned char most_space[];
+  T* most = reinterpret_cast<T*>(most_space);  // TOP: the maximum of each of the block's vectors
   __shared__ std::conditional_t<TOP, TopSpace, int> space;
   __shared__ Sums peers[kMaxCluster];
   __shared__ uint64_t peer_top[TOP ? kMaxCluster * kMaxTop : 1];
@@ -516,23 +537,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
   const int per = (row.vectors + C - 1) / C;
   const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
   Running<T, true, false> run(scale_of(p));
-  float best_max = -kInf;
-  uint4 best = make_uint4(0, 0, 0, 0);
-  int at = -1;
   const int64_t t = rank == 0 && threadIdx.x == 0 ? p.targets[r] : -1;
   each_vectors(row, v0, v1, [&](const uint4* raw, int v) {
     float top = -kInf;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
       const float m = Vec<T>::max(raw[u]);
-      if (TOP && v + u * kThreads < v1) {
-        most[v + u * kThreads - v0] = m;
-        if (m > best_max || at < 0) {
-          best_max = m;
-          best = raw[u];
-          at = v + u * kThreads;
-        }
-      }
+      if (TOP && v + u * kThreads < v1) most[v + u * kThreads - v0] = from_f32<T>(m);
       top = fmaxf(top, m);
     }
     run.see(top);
@@ -543,7 +554,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
   if (singles && threadIdx.x < row.singles) run.add_single(to_f32(row.x[row.single(threadIdx.x)]), false);
   const float target = t >= 0 && t < row.V ? to_f32(row.x[t]) : 0.f;
   Sums a = merge_block<true, false>(run.sums(), run.c);
-  if constexpr (TOP) block_top(space, row, v0, v1, singles, most, p.top_k, best, at);
+  if constexpr (TOP) block_top(space, row, v0, v1, singles, most, p.top_k);
   if (C > 1) {
     cluster_wait();  // every block has begun
     if (threadIdx.x == 0) *in_block(&peers[rank], 0) = a;
@@ -553,7 +564,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
     cluster_wait();
     if (rank != 0) return;
     a = merge_lanes<true, false>(peers[threadIdx.x % C], run.c, C);
-    if constexpr (TOP) rank_list(peer_top, C * kMaxTop, p.top_k, space.top);
+    if constexpr (TOP) merge_lists(peer_top, C, p.top_k, space.top);
   }
   const Stats st = finish<T, true, false>(p, row, a, [](int) { return false; });
   if (threadIdx.x == 0) {
@@ -987,7 +998,7 @@ cudaError_t by_type(int dtype, F f) {
 cudaError_t launch_token_logprobs(int dtype, const LogitsArgs& p, cudaStream_t stream) {
   return by_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    if (p.top_k > 0) return launch_rows(token_logprobs_kernel<T, true>, p, Vec<T>::E, (int)sizeof(float), stream);
+    if (p.top_k > 0) return launch_rows(token_logprobs_kernel<T, true>, p, Vec<T>::E, (int)sizeof(T), stream);
     return launch_rows(token_logprobs_kernel<T, false>, p, Vec<T>::E, 0, stream);
   });
 }
