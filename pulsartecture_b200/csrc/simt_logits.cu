@@ -42,6 +42,7 @@ constexpr int kMaxCluster = 8;  // the largest portable cluster
 constexpr int kMaxTop = 32;     // as fakla_token_logprobs takes; also the lanes of a warp
 constexpr int kMaxEntries = 256;  // as fakla_distill_topk takes
 constexpr int kCandidates = 512;
+constexpr int kOneWarp = 16;
 constexpr float kInf = __builtin_huge_valf();
 constexpr float kNaN = __builtin_nanf("");
 constexpr float kLog2e = 1.44269504f;
@@ -369,13 +370,16 @@ __device__ __forceinline__ float key_value(uint64_t k) {
 }
 
 // The pass that sums a row leaves the maximum of each vector in shared memory.
-// Of the 32 lanes, each with the largest maximum that it has in any warp, the
-// k-th largest has k values at or above it, so only values from there up can be
-// among the k largest: some 5 for k = 5 and 130 for k = 32 in a random row. They
-// are in the vectors whose maximum reaches it; those are listed first and then
-// read again all at once, by a thread per value. Keys, which hold the index too,
-// differ even between equal values, so rows of ties fill no list: lanes
-// interleave finely, and a row of one value lists its first 256 or so.
+// The k-th largest of the threads' own largest maxima has k values at or above
+// it, so only values from there up can be among the k largest: some 5 for k = 5
+// and 37 for k = 32 in a random row. Up to kOneWarp the threads of a lane go
+// together, and one warp finds the k-th of 32: 8192 x 32000 bf16 with k = 5
+// takes 123 us so and 127 us from 128 keys; with k = 32 that leaves 130
+// candidates, and 301 x 50257 fp32 takes 34 us so and 28 us from 128. They are in the vectors whose maximum
+// reaches it; those are listed first and then read again all at once, by a
+// thread per value. Keys, which hold the index too, differ even between equal
+// values, so rows of ties fill no list: threads interleave finely, and a row of
+// one value lists its first 256 or so.
 struct TopSpace {
   uint64_t best[kWarps][32];
   uint64_t list[kCandidates];
@@ -430,23 +434,39 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int k, ui
   __syncthreads();
 }
 
+// The keys of a warp in descending order over its lanes, by exchanges over
+// growing and shrinking distances (a bitonic network).
+__device__ __forceinline__ uint64_t sort_warp(uint64_t key) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int run = 2; run <= 32; run *= 2)
+#pragma unroll
+    for (int o = run / 2; o > 0; o /= 2) {
+      const uint64_t other = __shfl_xor_sync(~0u, key, o);
+      const bool larger = ((lane & o) == 0) == ((lane & run) == 0);  // this lane keeps the larger one
+      key = (other > key) == larger ? other : key;
+    }
+  return key;
+}
+
+// How many of 32 keys in descending order are above `key` (or equal to it).
+__device__ __forceinline__ int count_above(const uint64_t* list, uint64_t key, bool or_equal) {
+  int n = 0;
+#pragma unroll
+  for (int step = 16; step > 0; step /= 2)
+    if (list[n + step - 1] > key || (or_equal && list[n + step - 1] == key)) n += step;
+  return n + (list[n] > key || (or_equal && list[n] == key));
+}
+
 // The k largest of C blocks' top keys, each in descending order (kMaxTop
 // apart), into top: a key's rank is its place in its own list and the number of
-// larger ones in each other, found by halving.
+// larger ones in each other.
 __device__ __forceinline__ void merge_lists(const uint64_t* lists, int C, int k, uint64_t* top) {
   for (int i = threadIdx.x; i < C * k; i += kThreads) {
     const int own = i / k;
     const uint64_t key = lists[own * kMaxTop + (i - own * k)];
     int above = 0;
-    for (int c = 0; c < C; ++c) {
-      const uint64_t* list = lists + c * kMaxTop;
-      int larger = 0;
-#pragma unroll
-      for (int step = kMaxTop / 2; step > 0; step /= 2)
-        if (list[larger + step - 1] > key) larger += step;
-      larger += list[larger] > key;
-      above += larger;
-    }
+    for (int c = 0; c < C; ++c) above += count_above(lists + c * kMaxTop, key, false);
     if (above < k) top[above] = key;
   }
   __syncthreads();
@@ -467,17 +487,25 @@ __device__ __forceinline__ void block_top(TopSpace& sp, const Row<T>& row, int v
     }
   }
   uint64_t key = at < 0 ? 0 : order_key(best, row.lead + at * Row<T>::E + Row<T>::E - 1);
-  sp.best[threadIdx.x / 32][threadIdx.x % 32] = key;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   if (threadIdx.x == 0) sp.count = sp.vector_count = 0;
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    for (int w = 0; w < kWarps; ++w) key = sp.best[w][threadIdx.x] > key ? sp.best[w][threadIdx.x] : key;
-    int above = 0;  // its rank among the lanes; those without a value share key 0, in the order of the lanes
-#pragma unroll
-    for (int o = 0; o < 32; ++o) {
-      const uint64_t other = __shfl_sync(~0u, key, o);
-      above += other > key || (other == key && o < threadIdx.x);
+  // Those without a vector share key 0, in the order of the threads: the k-th
+  // is one of them where fewer have any, and then every value qualifies.
+  if (k <= kOneWarp) {
+    sp.best[warp][lane] = key;
+    __syncthreads();
+    if (warp == 0) {
+      for (int w = 1; w < kWarps; ++w) key = sp.best[w][lane] > key ? sp.best[w][lane] : key;
+      key = sort_warp(key);
+      if (lane == k - 1) sp.floor = key;
     }
+  } else {
+    key = sort_warp(key);
+    sp.best[warp][lane] = key;
+    __syncthreads();
+    int above = lane;
+    for (int w = 0; w < kWarps; ++w)
+      if (w != warp) above += count_above(sp.best[w], key, w < warp);
     if (above == k - 1) sp.floor = key;
   }
   __syncthreads();
@@ -955,7 +983,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
 // Blocks of a cluster, which share a row: as many as give every SM kBlocks,
 // while a thread keeps a vector or two, and as a block's shared memory asks for
 // (`bytes` per vector).
-constexpr int kBlocks = 6;
+constexpr int kBlocks = 4;
 int cluster_size(int64_t rows, int64_t vectors, int bytes) {
   int c = 1;
   while (c < kMaxCluster && ((rows * c < kBlocks * fakla_sm_count() && vectors / (2 * c) >= kThreads) ||
