@@ -234,9 +234,10 @@ struct Running {
 
 // Runs f(vectors, the first one's number) on every thread's vectors of
 // [v0, v1), kUnroll at a time, kThreads apart; the next ones are on their way
-// meanwhile. Past v1 the values are -inf, which add nothing.
-template <typename T, typename F>
-__device__ __forceinline__ void each_vectors(const Row<T>& row, int v0, int v1, F f) {
+// meanwhile. Past v1 the values are -inf, which add nothing. `first` is done
+// while the first of them are on their way.
+template <typename T, typename G, typename F>
+__device__ __forceinline__ void each_vectors(const Row<T>& row, int v0, int v1, G first, F f) {
   auto fetch = [&](uint4* raw, int v) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -249,6 +250,7 @@ __device__ __forceinline__ void each_vectors(const Row<T>& row, int v0, int v1, 
   uint4 even[kUnroll], odd[kUnroll];
   int v = v0 + threadIdx.x;
   fetch(even, v);
+  first();
   while (v < v1) {
     fetch(odd, v + step);
     f(even, v);
@@ -566,7 +568,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
   const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
   Running<T, true, false> run(scale_of(p));
   const int64_t t = rank == 0 && threadIdx.x == 0 ? p.targets[r] : -1;
-  each_vectors(row, v0, v1, [&](const uint4* raw, int v) {
+  each_vectors(row, v0, v1, [] {}, [&](const uint4* raw, int v) {
     float top = -kInf;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -626,10 +628,11 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
 // ---------------------------------------------------------------------------
 constexpr int kRound = kUnroll * kThreads;  // vectors of a block's loads in flight
 
-// Writes f(pair of logits) over the block's vectors [v0, v1) of a row. Stores
-// are as wide as the loads where both rows lie alike.
-template <typename T, typename F>
-__device__ __forceinline__ void map_vectors(const Row<T>& row, T* out, int v0, int v1, bool zero, F f) {
+// Writes f(pair of logits) over the block's vectors [v0, v1) of a row, or zeros.
+// Stores are as wide as the loads where both rows lie alike. `first` is done
+// while the first loads are on their way, not with zeros.
+template <typename T, typename G, typename F>
+__device__ __forceinline__ void map_vectors(const Row<T>& row, T* out, int v0, int v1, bool zero, G first, F f) {
   const bool wide = (((uintptr_t)row.x ^ (uintptr_t)out) & 15) == 0;
   auto put = [&](uint4 got, int v) {
     T* to = out + row.lead + v * Row<T>::E;
@@ -645,7 +648,7 @@ __device__ __forceinline__ void map_vectors(const Row<T>& row, T* out, int v0, i
     for (int v = v0 + threadIdx.x; v < v1; v += kThreads) put(make_uint4(0, 0, 0, 0), v);
     return;
   }
-  each_vectors(row, v0, v1, [&](const uint4* raw, int v) {
+  each_vectors(row, v0, v1, first, [&](const uint4* raw, int v) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
       if (v + u * kThreads < v1) {
@@ -695,7 +698,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
     const uint64_t f2 = sm100::f2_splat(flat), s2 = sm100::f2_splat(slope);
     const float low = -kFar / st.c;
     auto map = [&](auto sloped) {
-      map_vectors(row, out, v0, v1, zero, [&](const uint4& raw, int i) {
+      map_vectors(row, out, v0, v1, zero, [] {}, [&](const uint4& raw, int i) {
         uint4 v = raw;
         if constexpr (decltype(sloped)::value) v = Vec<T>::at_least(raw, low);  // p log p is 0 there
         const uint64_t l = sm100::f2_add(sm100::f2_fma(Vec<T>::pair(v, i), c2, nM), nl);
@@ -755,7 +758,8 @@ struct Entries {
   int id[kPerThread];  // -1: none
   float logit[kPerThread];
   bool bad;            // one of them is out of range
-  __device__ Entries(const LogitsArgs& p, uint32_t r) : bad(false) {
+  __device__ __forceinline__ void read(const LogitsArgs& p, uint32_t r) {
+    bad = false;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       const int k = threadIdx.x + i * kThreads;
@@ -832,27 +836,30 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   const Row<T> row(p, r);
   const int per = (row.vectors + C - 1) / C;
   const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
-  const Entries entries(p, r);
-  float given[kPerThread];  // the model's logits there
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) given[i] = rank == 0 && entries.id[i] >= 0 ? to_f32(row.x[entries.id[i]]) : 0.f;
-  if constexpr (REST) {
-    for (int i = threadIdx.x; i < (v1 - v0 + 3) / 4; i += kThreads) marks[i] = 0;
-    if (threadIdx.x == 0) single_marks = 0;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      const int id = entries.id[i];
-      if (id < 0) continue;
-      const int v = row.place(id);
-      if (v < 0) atomicOr(&single_marks, 1u << (-1 - v));
-      else if (v >= v0 && v < v1) atomicOr(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + (id - row.lead) % Row<T>::E));
-    }
-    __syncthreads();
-  }
   Running<T, false, REST> run(scale_of(p));
   const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
-  each_vectors(row, v0, v1, [&](const uint4* raw, int v) {
+  Entries entries;
+  float given[kPerThread];  // the model's logits there
+  auto first = [&] {
+    entries.read(p, r);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) given[i] = rank == 0 && entries.id[i] >= 0 ? to_f32(row.x[entries.id[i]]) : 0.f;
+    if constexpr (REST) {
+      for (int i = threadIdx.x; i < (v1 - v0 + 3) / 4; i += kThreads) marks[i] = 0;
+      if (threadIdx.x == 0) single_marks = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kPerThread; ++i) {
+        const int id = entries.id[i];
+        if (id < 0) continue;
+        const int v = row.place(id);
+        if (v < 0) atomicOr(&single_marks, 1u << (-1 - v));
+        else if (v >= v0 && v < v1) atomicOr(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + (id - row.lead) % Row<T>::E));
+      }
+      __syncthreads();
+    }
+  };
+  each_vectors(row, v0, v1, first, [&](const uint4* raw, int v) {
     float top = -kInf;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, Vec<T>::max(raw[u]));
@@ -923,27 +930,31 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   const float g = p.dloss[r] * p.inv_temperature;
   // dlogits_j = p_j outer, or for an entry p_j inner - its q
   const float inner = keep[4] * g, outer = (keep[4] - keep[5]) * g;
-  const Entries entries(p, r);
+  Entries entries;
   float given[kPerThread];
   bool mine[kPerThread];  // this block writes it
+  auto first = [&] {
+    entries.read(p, r);
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    float lq;
-    const int k = threadIdx.x + i * kThreads;
-    q_of[k] = teacher_q(p, entries.id[i], entries.logit[i], keep[2], keep[3], lq);
-    id_of[k] = entries.id[i];
-    mine[i] = entries.id[i] >= 0 && writes(row, entries.id[i], chunk, v0, v1);
-    given[i] = mine[i] ? to_f32(row.x[entries.id[i]]) : 0.f;
-  }
+    for (int i = 0; i < kPerThread; ++i) {
+      float lq;
+      const int k = threadIdx.x + i * kThreads;
+      q_of[k] = teacher_q(p, entries.id[i], entries.logit[i], keep[2], keep[3], lq);
+      id_of[k] = entries.id[i];
+      mine[i] = entries.id[i] >= 0 && writes(row, entries.id[i], chunk, v0, v1);
+      given[i] = mine[i] ? to_f32(row.x[entries.id[i]]) : 0.f;
+    }
+  };
   auto prob = [&](float x) { return exp2_approx(st.y(x) - st.l2s); };
   const bool zero = g == 0.f || (st.empty() && !isnan(inner));
   if (st.far) {
+    first();
     for (int j = row.lead + v0 * Row<T>::E + threadIdx.x; j < row.lead + v1 * Row<T>::E; j += kThreads)
       out[j] = from_f32<T>(zero ? 0.f : prob(to_f32(row.x[j])) * outer);
   } else {
     const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
     const uint64_t o2 = sm100::f2_splat(outer);
-    map_vectors(row, out, v0, v1, zero, [&](const uint4& raw, int i) {
+    map_vectors(row, out, v0, v1, zero, first, [&](const uint4& raw, int i) {
       const float2 f = sm100::f2_split(sm100::f2_add(sm100::f2_fma(Vec<T>::pair(raw, i), c2, nM), nl));
       return sm100::f2_mul(sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y))), o2);
     });
