@@ -404,8 +404,8 @@ int fakla_decode_noalloc(const void* q, const void* k, const void* v,
  *               may be state_in
  *   saved     : fakla_gated_scan_saved_bytes() that the backward reads, or NULL
  * h is carried in fp32. A gate of -inf (sigmoid) or 0 (identity) starts a new
- * sequence at its token. Identity gates are decay factors: products of 128
- * consecutive ones have to fit fp32.
+ * sequence at its token. Identity gates are decay factors: products of up to
+ * 64 consecutive ones have to fit fp32.
  */
 int fakla_gated_scan(const void* x, const void* gate, void* out, const float* state_in,
                      float* state_out, void* saved, int64_t B, int64_t T, int64_t D,

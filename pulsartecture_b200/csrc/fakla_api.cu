@@ -11,6 +11,7 @@
 #include <string.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <mutex>
 
 #include "fakla_common.cuh"
@@ -744,6 +745,31 @@ int check_gated_scan(int64_t B, int64_t T, int64_t D, int act, int dtype) {
                            (long long)D);
   return FAKLA_OK;
 }
+
+// Every pointer on a multiple of its element (null is).
+int check_elements(std::initializer_list<const void*> values, std::initializer_list<const void*> floats, int dtype) {
+  for (const void* p : values)
+    if ((uintptr_t)p % esize(dtype)) return fakla_set_error(FAKLA_ERR_ALIGNMENT, "a tensor does not start on an element");
+  for (const void* p : floats)
+    if ((uintptr_t)p % sizeof(float)) return fakla_set_error(FAKLA_ERR_ALIGNMENT, "an fp32 tensor does not start on an element");
+  return FAKLA_OK;
+}
+
+// The strides of a dimension of one row do not matter: 0 keeps every alignment.
+void set_inputs(fakla::GatedScanArgs* p, const void* x, const void* gate, int64_t B, int64_t T, int64_t D,
+                int64_t x_batch, int64_t x_time, int64_t gate_batch, int64_t gate_time, int act, int mix) {
+  p->x = x;
+  p->gate = gate;
+  p->x_batch = B > 1 ? x_batch : 0;
+  p->x_time = T > 1 ? x_time : 0;
+  p->gate_batch = B > 1 ? gate_batch : 0;
+  p->gate_time = T > 1 ? gate_time : 0;
+  p->B = B;
+  p->T = T;
+  p->D = D;
+  p->act = act;
+  p->mix = mix != 0;
+}
 }  // namespace
 
 extern "C" size_t fakla_gated_scan_saved_bytes(int64_t B, int64_t T, int64_t D) {
@@ -758,21 +784,12 @@ extern "C" int fakla_gated_scan(const void* x, const void* gate, void* out, cons
   int rc = check_gated_scan(B, T, D, act, dtype);
   if (rc) return rc;
   if (!x || !gate || !out) return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate and out must be non-NULL");
+  if ((rc = check_elements({x, gate, out}, {state_in, state_out, saved}, dtype))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};
   p.status = d->st();
-  p.x = x;
-  p.gate = gate;
-  p.x_batch = x_batch_stride;
-  p.x_time = x_time_stride;
-  p.gate_batch = gate_batch_stride;
-  p.gate_time = gate_time_stride;
-  p.B = B;
-  p.T = T;
-  p.D = D;
-  p.act = act;
-  p.mix = mix != 0;
+  set_inputs(&p, x, gate, B, T, D, x_batch_stride, x_time_stride, gate_batch_stride, gate_time_stride, act, mix);
   p.state_in = state_in;
   p.state_out = state_out;
   p.out = out;
@@ -791,21 +808,12 @@ extern "C" int fakla_gated_scan_backward(const void* x, const void* gate, const 
   if (rc) return rc;
   if (!x || !gate || !saved || !dout || !dx || !dgate)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate, saved, dout, dx and dgate must be non-NULL");
+  if ((rc = check_elements({x, gate, dout, dx, dgate}, {saved, dstate_out, dstate_in}, dtype))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};
   p.status = d->st();
-  p.x = x;
-  p.gate = gate;
-  p.x_batch = x_batch_stride;
-  p.x_time = x_time_stride;
-  p.gate_batch = gate_batch_stride;
-  p.gate_time = gate_time_stride;
-  p.B = B;
-  p.T = T;
-  p.D = D;
-  p.act = act;
-  p.mix = mix != 0;
+  set_inputs(&p, x, gate, B, T, D, x_batch_stride, x_time_stride, gate_batch_stride, gate_time_stride, act, mix);
   p.saved = (float*)const_cast<void*>(saved);
   p.dout = dout;
   p.dstate_out = dstate_out;
@@ -824,19 +832,12 @@ extern "C" int fakla_gated_scan_step(const void* x, const void* gate, void* out,
   if (rc) return rc;
   if (!x || !gate || !out || !state_in || !state_out)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate, out, state_in and state_out must be non-NULL");
+  if ((rc = check_elements({x, gate, out}, {state_in, state_out}, dtype))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};
   p.status = d->st();
-  p.x = x;
-  p.gate = gate;
-  p.x_batch = x_stride;
-  p.gate_batch = gate_stride;
-  p.B = N;
-  p.T = 1;
-  p.D = D;
-  p.act = act;
-  p.mix = mix != 0;
+  set_inputs(&p, x, gate, N, 1, D, x_stride, 0, gate_stride, 0, act, mix);
   p.state_in = state_in;
   p.state_out = state_out;
   p.out = out;
@@ -858,6 +859,7 @@ int check_logits(const void* logits, int64_t batch, int64_t rows, int64_t vocab,
   int rc = check_dtype(dtype);
   if (rc) return rc;
   if (!logits) return fakla_set_error(FAKLA_ERR_INVALID_ARG, "logits must be non-NULL");
+  if ((rc = check_elements({logits}, {}, dtype))) return rc;
   if (batch < 1 || rows < 1 || vocab < 1)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG, "sizes must be positive (batch=%lld rows=%lld vocab=%lld)",
                            (long long)batch, (long long)rows, (long long)vocab);
@@ -932,6 +934,7 @@ extern "C" int fakla_token_logprobs_backward(const void* logits, const int64_t* 
   if (!targets || !stats || !entropy || !dlogits || (dtop_logprobs && (!top_ids || top_k == 0)))
     return fakla_set_error(FAKLA_ERR_INVALID_ARG,
                            "targets, stats, entropy, dlogits and (with dtop_logprobs) top_ids must be non-NULL");
+  if ((rc = check_elements({dlogits}, {}, dtype))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   p.batch_stride = batch_stride;
@@ -989,6 +992,7 @@ extern "C" int fakla_distill_topk_backward(const void* logits, const int64_t* te
   if (!teacher_ids || !teacher_logits || !stats || !dloss || !dlogits)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG,
                            "teacher_ids, teacher_logits, stats, dloss and dlogits must be non-NULL");
+  if ((rc = check_elements({dlogits}, {}, dtype))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   p.batch_stride = batch_stride;

@@ -203,8 +203,7 @@ __device__ __forceinline__ float bounded(float A) { return fminf(fmaxf(A, -FLT_M
 
 __device__ __forceinline__ void cluster_sync() {
   __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  sm100::cluster_sync();
 }
 
 // One block's place: its channels of its batch row, and its rank in time.
@@ -238,7 +237,7 @@ struct Place {
 // of its tile, stored into all of them with the bytes counted on the receiver's
 // barrier, so a round costs one trip between SMs and no fence (a cluster
 // barrier per round, which also waits for the block's own global stores, took
-// 25 % longer). Two rounds' worth: a block gets a round's last value
+// 17 % longer). Two rounds' worth: a block gets a round's last value
 // from a peer only after that peer has read the round before.
 struct Exchange {
   float2 tiles[2][kMaxCluster][128];

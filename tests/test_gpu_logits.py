@@ -438,7 +438,7 @@ def test_captured_and_on_another_stream(cuda):
     in one case and not in the other."""
     from pulsartecture_b200 import distill_topk, token_logprobs
 
-    for rows, V in ((3, 20000), (900, 1111)):
+    for rows, V in ((3, 20000), (900, 1111), (600, 140000)):
         def inputs(seed):
             ids, top, lse, full = _teacher((rows,), V, 12, seed, 1.0)
             return [t.to(cuda) for t in (full.bfloat16(), ids[:, 3].contiguous(), ids, top, lse)]

@@ -37,6 +37,11 @@ def test_gated_scan_arguments():
     assert back(saved=None) == 1 and back(dx=None) == 1 and back(D=0) == 1 and back() in (4, 7)
     assert L.fakla_gated_scan_step(P, P, P, None, P, 1, 8, 8, 8, 5, 1, 1, None) == 1
     assert L.fakla_gated_scan_step(P, P, P, P, None, 1, 8, 8, 8, 5, 1, 1, None) == 1
+    odd = ctypes.c_void_p(17)
+    for bad in (dict(x=odd), dict(gate=odd), dict(out=odd)):
+        assert scan(**bad) == 3, bad
+    assert back(saved=odd) == 3 and back(dx=odd) == 3
+    assert L.fakla_gated_scan_step(P, P, P, P, odd, 1, 8, 8, 8, 5, 1, 1, None) == 3
     assert L.fakla_gated_scan_saved_bytes(2, 129, 10) >= 2 * 10 * 4
     assert L.fakla_gated_scan_saved_bytes(0, 129, 10) == 0
 
@@ -53,6 +58,7 @@ def test_logits_arguments():
                 dict(V=0), dict(k=-1), dict(k=33), dict(V=3), dict(temperature=0.0), dict(temperature=float("nan")),
                 dict(temperature=float("inf")), dict(temperature=-1.0), dict(dtype=2)):
         assert score(**bad) == 1, bad
+    assert score(logits=ctypes.c_void_p(18)) == 3  # fp32 from an address off 4 bytes
     assert score(V=2 ** 20 + 1) == 2 and score(rows=2 ** 40) == 2 and score(batch=2 ** 20, rows=2 ** 20) == 2
     assert score() in (4, 7) and score(k=0, top=None) in (4, 7)
 
