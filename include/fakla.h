@@ -538,7 +538,8 @@ int fakla_distill_topk_backward(const void* logits, const int64_t* teacher_ids,
 /*
  * fakla_device_status -- synchronise `stream` and return (then clear) the
  * device-side status word that kernels set when a bounded wait expires
- * (FAKLA_ERR_TIMEOUT) or a device-side check fails. FAKLA_OK if clean.
+ * (FAKLA_ERR_TIMEOUT) or a device-side check fails (FAKLA_ERR_INVALID_ARG: a
+ * token id outside of the vocabulary). FAKLA_OK if clean.
  */
 int fakla_device_status(void* stream);
 
