@@ -47,7 +47,8 @@ namespace {
 
 constexpr int kWarps = 8;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxCluster = 8;  // the largest portable cluster
+constexpr int kPortableCluster = 8;
+constexpr int kMaxCluster = 16;
 // Tokens per thread and round. The forward holds a and b of a run and the next
 // round's raw values, the backward a, 1 - a, h, and the raw x and dout: with
 // four channels both fit 128 registers, two blocks on an SM.
@@ -605,10 +606,13 @@ __global__ void __launch_bounds__(kThreads) scan_step_kernel(GatedScanArgs p) {
 
 // Runs f with the type, channels per thread, gate activation and input form as
 // constants. Channels go in fours (bf16) or twos where every row starts on a
-// multiple of their size, and, for the scans, where blocks still reach every SM:
-// at `most` of them share a warp's channels (0: no such limit).
+// multiple of their size, and, for a scan of `tiles` tiles (0: one token), where
+// the blocks then still reach every SM: 8 bytes of channels with 8 blocks on a
+// sequence, 4 bytes with 16. bf16 forward, one / two / four channels a thread:
+// 1 x 8192 x 512 takes 21 / 22 / 25 us, 1 x 16384 x 1024 73 / 54 / 57,
+// 4 x 2048 x 512 21 / 14 / 17, 64 x 64 x 1024 13 / 11 / 9.
 template <typename F>
-void dispatch(int dtype, const GatedScanArgs& p, int64_t most, F f) {
+void dispatch(int dtype, const GatedScanArgs& p, int64_t tiles, F f) {
   auto by_form = [&](auto t, auto vec, auto a) {
     if (p.mix) f(t, vec, a, std::true_type{}); else f(t, vec, a, std::false_type{});
   };
@@ -620,7 +624,9 @@ void dispatch(int dtype, const GatedScanArgs& p, int64_t most, F f) {
   const uintptr_t bases = (uintptr_t)p.x | (uintptr_t)p.gate | (uintptr_t)p.out | (uintptr_t)p.dout |
                           (uintptr_t)p.dx | (uintptr_t)p.dgate;
   auto fits = [&](int vec, int bytes) {
-    return steps % vec == 0 && bases % (vec * bytes) == 0 && (most == 0 || p.B * (p.D / (32 * vec)) * most >= fakla_sm_count());
+    if (steps % vec != 0 || bases % (vec * bytes) != 0) return false;
+    const int64_t most = vec * bytes == 8 ? kPortableCluster : kMaxCluster;
+    return tiles == 0 || p.B * (p.D / (32 * vec)) * (tiles < most ? tiles : most) >= fakla_sm_count();
   };
   if (dtype == FAKLA_BF16) {
     if (fits(4, 2)) by_act(__nv_bfloat16{}, std::integral_constant<int, 4>{});
@@ -636,7 +642,8 @@ void dispatch(int dtype, const GatedScanArgs& p, int64_t most, F f) {
 // five blocks, and no more than there are tiles. More blocks fill the SMs but
 // wait longer for one another: 8 x 4096 x 2048 bf16 takes 104 us with 2 and
 // 109 with 4, 3 x 1001 x 515 fp32 (forward and backward) 23 us with 4 and 28
-// with 8, 65536 x 4096 bf16 434 us with 8 and 710 with 4.
+// with 8, 65536 x 4096 bf16 434 us with 8, 710 with 4 and 633 with 16,
+// 65536 x 64 95 us with 16 and 169 with 8.
 int cluster_size(int64_t groups, int64_t tiles) {
   int c = 1;
   while (c < kMaxCluster && 2 * c <= tiles && groups * c * 4 < (int64_t)fakla_sm_count() * 5) c *= 2;
@@ -644,15 +651,14 @@ int cluster_size(int64_t groups, int64_t tiles) {
 }
 
 template <typename K>
-cudaError_t launch(K kernel, const GatedScanArgs& p, int vec, int tile, cudaStream_t stream) {
+cudaError_t launch(K kernel, const GatedScanArgs& p, int vec, int64_t tiles, cudaStream_t stream) {
   const int64_t groups = p.B * ((p.D + 32 * vec - 1) / (32 * vec));
-  const int c = cluster_size(groups, (p.T + tile - 1) / tile);
+  const int c = cluster_size(groups, tiles);
+  if (c > kPortableCluster) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
   return launch_chained(kernel, dim3((unsigned)(groups * c)), dim3(kThreads), 0, stream, (unsigned)c, p, c);
-}
-
-int64_t most_blocks(const GatedScanArgs& p, int tile) {
-  const int64_t tiles = (p.T + tile - 1) / tile;
-  return tiles < kMaxCluster ? tiles : kMaxCluster;
 }
 
 }  // namespace
@@ -663,17 +669,19 @@ size_t gated_scan_saved_bytes(int64_t B, int64_t T, int64_t D) {
 
 cudaError_t launch_gated_scan(int dtype, const GatedScanArgs& p, cudaStream_t stream) {
   constexpr int kTile = kWarps * kForwardRun;
+  const int64_t tiles = (p.T + kTile - 1) / kTile;
   cudaError_t e = cudaSuccess;
-  dispatch(dtype, p, most_blocks(p, kTile), [&](auto t, auto vec, auto act, auto mix) {
-    e = launch(scan_forward_kernel<decltype(t), vec(), act(), mix()>, p, vec(), kTile, stream);
+  dispatch(dtype, p, tiles, [&](auto t, auto vec, auto act, auto mix) {
+    e = launch(scan_forward_kernel<decltype(t), vec(), act(), mix()>, p, vec(), tiles, stream);
   });
   return e;
 }
 
 cudaError_t launch_gated_scan_backward(int dtype, const GatedScanArgs& p, cudaStream_t stream) {
+  const int64_t tiles = (p.T + kKept - 1) / kKept;
   cudaError_t e = cudaSuccess;
-  dispatch(dtype, p, most_blocks(p, kKept), [&](auto t, auto vec, auto act, auto mix) {
-    e = launch(scan_backward_kernel<decltype(t), vec(), act(), mix()>, p, vec(), kKept, stream);
+  dispatch(dtype, p, tiles, [&](auto t, auto vec, auto act, auto mix) {
+    e = launch(scan_backward_kernel<decltype(t), vec(), act(), mix()>, p, vec(), tiles, stream);
   });
   return e;
 }

@@ -40,7 +40,7 @@ def _close(got, value, bound, name):
 SIZES = [(1, 1, 1), (2, 1, 7), (1, 2, 64), (3, 5, 33), (1, 127, 8), (2, 128, 65), (2, 129, 130), (1, 1000, 515),
          (5, 257, 64), (1, 4100, 40), (40, 17, 192),
          # batches that put one, two and four blocks on a sequence
-         (300, 390, 33), (150, 520, 64), (75, 1100, 64)]
+         (300, 390, 33), (150, 520, 64), (75, 1100, 64), (2, 2111, 64), (10, 1030, 256)]
 
 
 @pytest.mark.parametrize("B,T,D", SIZES)
