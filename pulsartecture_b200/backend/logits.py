@@ -81,7 +81,7 @@ class _TokenLogprobsFn(torch.autograd.Function):
         rows, targets, stats, ent, ids = ctx.saved_tensors
         at, top_k, temperature, ignore_index, code, shape = ctx.form
         dlp, dent, dtop = (None if t is None else t.contiguous() for t in (dlp, dent, dtop))
-        dlogits = torch.empty(shape, device=rows.device, dtype=rows.dtype)
+        dlogits = torch.empty_like(rows, memory_format=torch.contiguous_format).view(shape)
         _launch(rows.device, _lib.lib().fakla_token_logprobs_backward, _ptr(rows), _ptr(targets), _ptr(stats), _ptr(ent),
                 _ptr(ids), _ptr(dlp), _ptr(dent), _ptr(dtop), _ptr(dlogits), *at, top_k, temperature, ignore_index, code)
         return dlogits, None, None, None, None, None
@@ -89,8 +89,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
 
 def _run_logprobs(rows, at, targets, top_k, temperature, ignore_index, code, save):
     dev, lead = rows.device, targets.shape
-    lp = torch.empty(lead, device=dev, dtype=torch.float32)
-    ent = torch.empty(lead, device=dev, dtype=torch.float32)
+    lp = torch.empty_like(targets, dtype=torch.float32)
+    ent = torch.empty_like(lp)
     top = torch.empty((*lead, top_k), device=dev, dtype=torch.float32) if top_k else None
     ids = torch.empty((*lead, top_k), device=dev, dtype=torch.int64) if top_k else None
     stats = torch.empty((at[0] * at[1], 2), device=dev, dtype=torch.float32) if save else None
@@ -159,7 +159,7 @@ class _DistillFn(torch.autograd.Function):
         rows, ids, teacher, lse, stats = ctx.saved_tensors
         at, temperature, code, shape = ctx.form
         dloss = dloss.contiguous()
-        dlogits = torch.empty(shape, device=rows.device, dtype=rows.dtype)
+        dlogits = torch.empty_like(rows, memory_format=torch.contiguous_format).view(shape)
         _launch(rows.device, _lib.lib().fakla_distill_topk_backward, _ptr(rows), _ptr(ids), _ptr(teacher), _ptr(lse),
                 _ptr(stats), _ptr(dloss), _ptr(dlogits), *at, ids.shape[-1], temperature, code)
         return dlogits, None, None, None, None, None

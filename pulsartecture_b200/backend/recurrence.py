@@ -72,10 +72,9 @@ class _GatedScanFn(torch.autograd.Function):
         act, mix, code, has_state = ctx.form
         B, T, D = x.shape
         dev = x.device
-        dx = torch.empty((B, T, D), device=dev, dtype=x.dtype)
-        dgate = torch.empty((B, T, D), device=dev, dtype=x.dtype)
+        dout = torch.zeros((B, T, D), device=dev, dtype=x.dtype) if dout is None else dout.contiguous()
+        dx, dgate = torch.empty_like(dout), torch.empty_like(dout)
         dstate = torch.empty((B, D), device=dev, dtype=torch.float32) if has_state else None
-        dout = torch.zeros_like(dx) if dout is None else dout.contiguous()
         dfinal = None if dfinal is None else dfinal.contiguous()
         xb, xt, _ = x.stride()
         gb, gt, _ = gate.stride()
@@ -88,7 +87,7 @@ def _run_scan(x, gate, state, act, mix, code, return_state, save):
     B, T, D = x.shape
     dev = x.device
     L = _lib.lib()
-    out = torch.empty((B, T, D), device=dev, dtype=x.dtype)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     final = torch.empty((B, D), device=dev, dtype=torch.float32) if return_state else None
     saved = torch.empty(L.fakla_gated_scan_saved_bytes(B, T, D), device=dev, dtype=torch.uint8) if save else None
     xb, xt, _ = x.stride()

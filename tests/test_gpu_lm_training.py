@@ -105,7 +105,7 @@ def test_padding_is_left_out(cuda):
     # sequence 0 whole and sequence 1 up to its end: the padding behind changes nothing
     a, b = model.loss(ids[:1]), model.loss(ids[1:, :20])
     assert torch.allclose(loss, (29 * a + 19 * b) / 48, rtol=1e-5, atol=1e-6)
-    assert float(model.loss(torch.full_like(ids, -100))) == 0.0
+    assert float(model.loss(torch.full_like(ids, -100)).detach()) == 0.0
     one = model.loss(ids[:, :1])  # no next token at all
     one.backward()
     assert float(one.detach()) == 0.0
