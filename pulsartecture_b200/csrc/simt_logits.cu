@@ -147,6 +147,7 @@ struct Sums {
   float s;  // sum 2^y
   float w;  // sum 2^y y
   float t;  // sum 2^y outside of the teacher's entries
+  float u;  // and at them
 };
 
 // M of a maximum m, kept finite for -inf.
@@ -161,11 +162,17 @@ __device__ __forceinline__ Sums merge_lanes(Sums a, float c, int width) {
   const float move = base_of(a.m, c) - base_of(m, c), f = exp2_approx(move);
   if (WEIGHTED) a.w = f * fmaf(move, a.s, a.w);
   a.s *= f;
-  if (REST) a.t *= f;
+  if (REST) {
+    a.t *= f;
+    a.u *= f;
+  }
   for (int o = width / 2; o > 0; o >>= 1) {
     a.s += __shfl_xor_sync(~0u, a.s, o);
     if (WEIGHTED) a.w += __shfl_xor_sync(~0u, a.w, o);
-    if (REST) a.t += __shfl_xor_sync(~0u, a.t, o);
+    if (REST) {
+      a.t += __shfl_xor_sync(~0u, a.t, o);
+      a.u += __shfl_xor_sync(~0u, a.u, o);
+    }
   }
   a.m = m;
   return a;
@@ -228,7 +235,7 @@ struct Running {
   }
   __device__ Sums sums() const {
     auto both = [](uint64_t v) { const float2 f = sm100::f2_split(v); return f.x + f.y; };
-    return {m, both(s2), WEIGHTED ? both(w2) : 0.f, REST ? both(t2) : 0.f};
+    return {m, both(s2), WEIGHTED ? both(w2) : 0.f, REST ? both(t2) : 0.f, 0.f};
   }
 };
 
@@ -294,6 +301,7 @@ struct Stats {
   float l2s;   // log2 s; +inf in a row of nothing but -inf, NaN in one with a NaN or +inf
   float mean;  // sum p y
   float rest;  // sum of p outside of the teacher's entries
+  float in;    // and at them
   bool far;    // y from (x - m) / temperature
   float c, inv_t;
   __device__ bool empty() const { return l2s == kInf; }
@@ -324,34 +332,36 @@ __device__ Stats finish(const LogitsArgs& p, const Row<T>& row, Sums a, F member
   Stats r = stats_of(p, a.m == -kInf ? 0.f : a.m, 0.f);
   const bool none = a.m == -kInf && !isnan(a.s);
   if (r.far) {  // the same for every thread
-    float s = 0.f, w = 0.f, t = 0.f;
+    float s = 0.f, w = 0.f, t = 0.f, u = 0.f;
     for (int j = threadIdx.x; j < row.V; j += kThreads) {
       const float y = (to_f32(row.x[j]) - r.m) * r.inv_t * kLog2e, e = exp2f(y);
       s += e;
       if (WEIGHTED) w += e == 0.f ? 0.f : e * y;
-      if (REST && !member(j)) t += e;
+      if (REST) (member(j) ? u : t) += e;
     }
-    __shared__ float part[3][kWarps];
-    float v[3] = {s, w, t};
-    for (int i = 0; i < 3; ++i) {
+    __shared__ float part[4][kWarps];
+    float v[4] = {s, w, t, u};
+    for (int i = 0; i < 4; ++i) {
       for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(~0u, v[i], o);
       if (threadIdx.x % 32 == 0) part[i][threadIdx.x / 32] = v[i];
     }
     __syncthreads();
-    a.s = a.w = a.t = 0.f;
+    a.s = a.w = a.t = a.u = 0.f;
     for (int i = 0; i < kWarps; ++i) {
       a.s += part[0][i];
       a.w += part[1][i];
       a.t += part[2][i];
+      a.u += part[3][i];
     }
   }
   if (none || a.s == 0.f) {
     r.l2s = kInf;
-    r.mean = r.rest = 0.f;
+    r.mean = r.rest = r.in = 0.f;
   } else {
     r.l2s = log2f(a.s);
     r.mean = a.w / a.s;
     r.rest = a.t / a.s;
+    r.in = a.u / a.s;
   }
   return r;
 }
@@ -841,10 +851,11 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
   Entries entries;
   float given[kPerThread];  // the model's logits there
+  bool fresh[kPerThread];   // the values of this block that are entries, each once
   auto first = [&] {
     entries.read(p, r);
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i) given[i] = rank == 0 && entries.id[i] >= 0 ? to_f32(row.x[entries.id[i]]) : 0.f;
+    for (int i = 0; i < kPerThread; ++i) given[i] = entries.id[i] >= 0 ? to_f32(row.x[entries.id[i]]) : 0.f;
     if constexpr (REST) {
       for (int i = threadIdx.x; i < (v1 - v0 + 3) / 4; i += kThreads) marks[i] = 0;
       if (threadIdx.x == 0) single_marks = 0;
@@ -852,10 +863,12 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
 #pragma unroll
       for (int i = 0; i < kPerThread; ++i) {
         const int id = entries.id[i];
+        fresh[i] = false;
         if (id < 0) continue;
         const int v = row.place(id);
-        if (v < 0) atomicOr(&single_marks, 1u << (-1 - v));
-        else if (v >= v0 && v < v1) atomicOr(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + (id - row.lead) % Row<T>::E));
+        auto claim = [&](uint32_t* word, uint32_t bit) { fresh[i] = !(atomicOr(word, bit) & bit); };
+        if (v >= v0 && v < v1) claim(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + (id - row.lead) % Row<T>::E));
+        else if (v < 0 && rank == 0) claim(&single_marks, 1u << (-1 - v));
       }
       __syncthreads();
     }
@@ -870,7 +883,14 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   });
   if (rank == 0 && threadIdx.x < row.singles)
     run.add_single(to_f32(row.x[row.single(threadIdx.x)]), REST && (single_marks >> threadIdx.x & 1));
-  Sums a = merge_block<false, REST>(run.sums(), run.c);
+  if constexpr (REST)
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) run.see(fresh[i] ? given[i] : -kInf);
+  Sums a = run.sums();
+  if constexpr (REST)
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) a.u += exp2_approx(fmaf(fresh[i] ? given[i] : -kInf, run.c, -run.M));
+  a = merge_block<false, REST>(a, run.c);
   if (C > 1) {
     cluster_wait();
     if (threadIdx.x == 0) *in_block(&peers[rank], 0) = a;
@@ -894,10 +914,15 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   }
   __syncthreads();
   loss = sum_block(loss);
-  float ratio = 0.f;  // q_r / p_r
+  // The rest as a class. With q_r = 1 - Q and p_r = 1 - P the ratio q_r / p_r is
+  // 1 + (P - Q) / p_r, whose difference keeps its digits where the entries hold
+  // little: there a quotient of two rounded sums near 1 is off by 10^-5 of the
+  // loss, this by 10^-7.
+  float outside = t.mass;  // what p outside of the entries is multiplied by: Q + q_r - q_r / p_r
   if (REST && t.rest > 0.f) {
-    ratio = t.rest / st.rest;
-    loss += t.rest * logf(ratio);
+    const float more = st.rest == 0.f ? kInf : (st.in - t.mass) / st.rest;
+    loss += t.rest * (fabsf(more) < 0.5f ? log1pf(more) : logf(t.rest / st.rest));
+    outside = isinf(more) ? 0.f : -more;  // infinite: every p outside is 0
   }
   if (threadIdx.x != 0) return;
   if (t.bad) {
@@ -912,7 +937,7 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
     keep[2] = t.m;
     keep[3] = t.logs;
     keep[4] = t.bad ? kNaN : t.mass + t.rest;
-    keep[5] = isinf(ratio) ? 0.f : ratio;  // infinite: every p outside of the entries is 0
+    keep[5] = t.bad ? kNaN : outside;
   }
 }
 
@@ -930,7 +955,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   const Stats st = stats_of(p, keep[0], keep[1]);
   const float g = p.dloss[r] * p.inv_temperature;
   // dlogits_j = p_j outer, or for an entry p_j inner - its q
-  const float inner = keep[4] * g, outer = (keep[4] - keep[5]) * g;
+  const float inner = keep[4] * g, outer = keep[5] * g;
   Entries entries;
   float given[kPerThread];
   bool mine[kPerThread];  // this block writes it

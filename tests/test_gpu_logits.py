@@ -368,6 +368,50 @@ def test_distill_repeated_ids_and_masks(cuda):
     _check_distill(cuda, logits[:2], ids[:2], top[:2], lse2[:2], 1.0)
 
 
+@pytest.mark.parametrize("rows,V", [(3, 2003), (2, 40001), (700, 1000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_small_divergences(cuda, rows, V, dtype):
+    """Entries that hold little: the rest's class, q_r log(q_r / p_r) with both
+    near 1, keeps its digits. Few rows are split over a cluster's blocks; one
+    entry is named twice, one lies at a row's unaligned end."""
+    from pulsartecture_b200 import distill_topk
+
+    T = 2.0
+    g = torch.Generator().manual_seed(V)
+    full = torch.randn(rows, V, generator=g)
+    logits = (full + 0.5 * torch.randn(rows, V, generator=g)).to(dtype)
+    ids = torch.tensor([V // 3, V - 1, V // 3, -1]).expand(rows, 4).contiguous()
+    top = full.gather(-1, ids.clamp_min(0))
+    lse = torch.logsumexp(full.double() / T, -1).float()
+    leaf = logits.to(cuda).requires_grad_()
+    dloss = torch.ones(rows)
+    want = O.distill(logits, ids, top, lse, T, dloss)
+    loss = distill_topk(leaf, ids.to(cuda), top.to(cuda), lse.to(cuda), temperature=T)
+    p = want["p"]
+    lp = torch.log(p)
+    # Q and P are off by their relative errors: the exponentials', 4u, and their
+    # arguments' (teacher: terms up to `size`; model: `err` and 4 |log p| u); the
+    # rest's class is q_r log1p((P - Q) / p_r), off by those of P and Q and, with
+    # q_r and p_r near 1, by 8u of itself, the entries' terms q (log q - log p)
+    # by q times both and 8u of themselves
+    err = _sum_error(V, lp, p)
+    q = torch.exp(top.double() / T - lse.double()[:, None])[:, :3]
+    Q, P = q.sum(-1), p[:, [V // 3, V - 1]].sum(-1)
+    assert float(Q.max()) < 0.03 and float(P.max()) < 0.03
+    size = (top.double().abs() / T).amax(-1) + lse.double().abs()
+    most = lp.abs().amax(-1)
+    rel_q, rel_p = U * (8 + 4 * size), err + U * (8 + 4 * most)
+    terms = (q * (torch.log(q) - lp.gather(-1, ids[:, :3]))).sum(-1).abs()
+    tol = 1.1 * (2 * (Q * rel_q + P * rel_p) + Q * (rel_q + rel_p)) + 8 * U * (terms + Q + P)
+    _within(loss, want["loss"], tol, "loss")
+    # a logit that is no entry: p_j (Q - P) / p_r, p_j's relative error and that of Q - P
+    got, = torch.autograd.grad(loss, leaf, dloss.to(cuda))
+    rest = torch.ones(V, dtype=torch.bool)
+    rest[ids[0, :3]] = False
+    off = p * (1.1 * (Q * rel_q + P * rel_p) + 8 * U * (Q + P))[:, None] + (rel_p[:, None] + 8 * U) * want["dlogits"].abs()
+    _within(got[:, rest], want["dlogits"][:, rest], off[:, rest] / T, "dlogits")
+
+
 def test_distill_rows_without_a_distribution(cuda):
     from pulsartecture_b200 import _lib, distill_topk
     from pulsartecture_b200.backend.interface import device_status
