@@ -146,8 +146,6 @@ struct Sums {
   float m;  // the largest value
   float s;  // sum 2^y
   float w;  // sum 2^y y
-  float t;  // sum 2^y outside of the teacher's entries
-  float u;  // and at them
 };
 
 // M of a maximum m, kept finite for -inf.
@@ -155,38 +153,29 @@ __device__ __forceinline__ float base_of(float m, float c) { return fmaxf(__fmul
 
 // The sums over `width` neighbouring lanes (a power of two), in each of them:
 // all are moved to the largest value's base once, then added in a fixed order.
-template <bool WEIGHTED, bool REST>
+template <bool WEIGHTED>
 __device__ __forceinline__ Sums merge_lanes(Sums a, float c, int width) {
   float m = a.m;
   for (int o = width / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
   const float move = base_of(a.m, c) - base_of(m, c), f = exp2_approx(move);
   if (WEIGHTED) a.w = f * fmaf(move, a.s, a.w);
   a.s *= f;
-  if (REST) {
-    a.t *= f;
-    a.u *= f;
-  }
   for (int o = width / 2; o > 0; o >>= 1) {
     a.s += __shfl_xor_sync(~0u, a.s, o);
     if (WEIGHTED) a.w += __shfl_xor_sync(~0u, a.w, o);
-    if (REST) {
-      a.t += __shfl_xor_sync(~0u, a.t, o);
-      a.u += __shfl_xor_sync(~0u, a.u, o);
-    }
   }
   a.m = m;
   return a;
 }
 
-// One thread's running sums. WEIGHTED: the entropy's; REST: those outside of
-// the teacher's entries.
-template <typename T, bool WEIGHTED, bool REST>
+// One thread's running sums. WEIGHTED: the entropy's.
+template <typename T, bool WEIGHTED>
 struct Running {
   static constexpr int E = Vec<T>::E;
   float m, M, c;
-  uint64_t c2, s2, w2, t2;
+  uint64_t c2, s2, w2;
   __device__ explicit Running(float c_) : m(-kInf), M(-kFar), c(c_), c2(sm100::f2_splat(c_)) {
-    s2 = w2 = t2 = sm100::f2_splat(0.f);
+    s2 = w2 = sm100::f2_splat(0.f);
   }
   __device__ __forceinline__ void see(float most) {
     if (most > m) {
@@ -195,47 +184,32 @@ struct Running {
       const uint64_t f = sm100::f2_splat(exp2_approx(M - to));
       if (WEIGHTED) w2 = sm100::f2_mul(f, sm100::f2_fma(sm100::f2_splat(M - to), s2, w2));
       s2 = sm100::f2_mul(f, s2);
-      if (REST) t2 = sm100::f2_mul(f, t2);
       M = to;
     }
   }
-  // member: bit i set where value i is one of the teacher's entries
-  __device__ __forceinline__ void add(uint4 v, uint32_t member) {
+  __device__ __forceinline__ void add(uint4 v) {
     if (WEIGHTED) v = Vec<T>::at_least(v, -kFar / c);  // 2^y y is 0 there, not 0 times -inf
     const uint64_t nM = sm100::f2_splat(-M);
-    uint64_t e[E / 2], all = 0;
+    uint64_t all = 0;
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) {
       const uint64_t y = sm100::f2_fma(Vec<T>::pair(v, i), c2, nM);
       const float2 f = sm100::f2_split(y);
-      e[i] = sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y)));
-      all = i == 0 ? e[i] : sm100::f2_add(all, e[i]);
-      if (WEIGHTED) w2 = sm100::f2_fma(e[i], y, w2);
+      const uint64_t e = sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y)));
+      all = i == 0 ? e : sm100::f2_add(all, e);
+      if (WEIGHTED) w2 = sm100::f2_fma(e, y, w2);
     }
     s2 = sm100::f2_add(s2, all);
-    if (REST) {
-      if (member == 0) {
-        t2 = sm100::f2_add(t2, all);
-      } else {
-#pragma unroll
-        for (int i = 0; i < E / 2; ++i) {
-          const float2 f = sm100::f2_split(e[i]);
-          t2 = sm100::f2_add(t2, sm100::f2_make(member >> (2 * i) & 1 ? 0u : __float_as_uint(f.x),
-                                                member >> (2 * i + 1) & 1 ? 0u : __float_as_uint(f.y)));
-        }
-      }
-    }
   }
-  __device__ __forceinline__ void add_single(float x, bool member) {
+  __device__ __forceinline__ void add_single(float x) {
     see(x);
     const float y = fmaf(WEIGHTED ? (x < -kFar / c ? -kFar / c : x) : x, c, -M), e = exp2_approx(y);
     s2 = sm100::f2_add(s2, sm100::f2_make(__float_as_uint(e), 0u));
     if (WEIGHTED) w2 = sm100::f2_fma(sm100::f2_make(__float_as_uint(e), 0u), sm100::f2_make(__float_as_uint(y), 0u), w2);
-    if (REST && !member) t2 = sm100::f2_add(t2, sm100::f2_make(__float_as_uint(e), 0u));
   }
   __device__ Sums sums() const {
     auto both = [](uint64_t v) { const float2 f = sm100::f2_split(v); return f.x + f.y; };
-    return {m, both(s2), WEIGHTED ? both(w2) : 0.f, REST ? both(t2) : 0.f, 0.f};
+    return {m, both(s2), WEIGHTED ? both(w2) : 0.f};
   }
 };
 
@@ -270,13 +244,13 @@ __device__ __forceinline__ void each_vectors(const Row<T>& row, int v0, int v1, 
 }
 
 // The sums over the block, in every thread.
-template <bool WEIGHTED, bool REST>
+template <bool WEIGHTED>
 __device__ __forceinline__ Sums merge_block(Sums a, float c) {
   __shared__ Sums part[kWarps];
-  a = merge_lanes<WEIGHTED, REST>(a, c, 32);
+  a = merge_lanes<WEIGHTED>(a, c, 32);
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = a;
   __syncthreads();
-  return merge_lanes<WEIGHTED, REST>(part[threadIdx.x % kWarps], c, kWarps);
+  return merge_lanes<WEIGHTED>(part[threadIdx.x % kWarps], c, kWarps);
 }
 
 __device__ __forceinline__ void cluster_arrive() {
@@ -300,8 +274,7 @@ struct Stats {
   float m, M;
   float l2s;   // log2 s; +inf in a row of nothing but -inf, NaN in one with a NaN or +inf
   float mean;  // sum p y
-  float rest;  // sum of p outside of the teacher's entries
-  float in;    // and at them
+  float s;     // sum 2^y (by `finish`)
   bool far;    // y from (x - m) / temperature
   float c, inv_t;
   __device__ bool empty() const { return l2s == kInf; }
@@ -326,42 +299,38 @@ __device__ __forceinline__ Stats stats_of(const LogitsArgs& p, float m, float l2
   return r;
 }
 
-// All threads of the block; `member(j)` is used with REST.
-template <typename T, bool WEIGHTED, bool REST, typename F>
-__device__ Stats finish(const LogitsArgs& p, const Row<T>& row, Sums a, F member) {
+// By all threads of the block.
+template <typename T, bool WEIGHTED>
+__device__ Stats finish(const LogitsArgs& p, const Row<T>& row, Sums a) {
   Stats r = stats_of(p, a.m == -kInf ? 0.f : a.m, 0.f);
   const bool none = a.m == -kInf && !isnan(a.s);
   if (r.far) {  // the same for every thread
-    float s = 0.f, w = 0.f, t = 0.f, u = 0.f;
+    float s = 0.f, w = 0.f;
     for (int j = threadIdx.x; j < row.V; j += kThreads) {
       const float y = (to_f32(row.x[j]) - r.m) * r.inv_t * kLog2e, e = exp2f(y);
       s += e;
       if (WEIGHTED) w += e == 0.f ? 0.f : e * y;
-      if (REST) (member(j) ? u : t) += e;
     }
-    __shared__ float part[4][kWarps];
-    float v[4] = {s, w, t, u};
-    for (int i = 0; i < 4; ++i) {
+    __shared__ float part[2][kWarps];
+    float v[2] = {s, w};
+    for (int i = 0; i < 2; ++i) {
       for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(~0u, v[i], o);
       if (threadIdx.x % 32 == 0) part[i][threadIdx.x / 32] = v[i];
     }
     __syncthreads();
-    a.s = a.w = a.t = a.u = 0.f;
+    a.s = a.w = 0.f;
     for (int i = 0; i < kWarps; ++i) {
       a.s += part[0][i];
       a.w += part[1][i];
-      a.t += part[2][i];
-      a.u += part[3][i];
     }
   }
+  r.s = a.s;
   if (none || a.s == 0.f) {
     r.l2s = kInf;
-    r.mean = r.rest = r.in = 0.f;
+    r.mean = 0.f;
   } else {
     r.l2s = log2f(a.s);
     r.mean = a.w / a.s;
-    r.rest = a.t / a.s;
-    r.in = a.u / a.s;
   }
   return r;
 }
@@ -577,7 +546,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
   const Row<T> row(p, r);
   const int per = (row.vectors + C - 1) / C;
   const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
-  Running<T, true, false> run(scale_of(p));
+  Running<T, true> run(scale_of(p));
   const int64_t t = rank == 0 && threadIdx.x == 0 ? p.targets[r] : -1;
   each_vectors(row, v0, v1, [] {}, [&](const uint4* raw, int v) {
     float top = -kInf;
@@ -589,12 +558,12 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
     }
     run.see(top);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) run.add(raw[u], 0);
+    for (int u = 0; u < kUnroll; ++u) run.add(raw[u]);
   });
   const bool singles = rank == 0;
-  if (singles && threadIdx.x < row.singles) run.add_single(to_f32(row.x[row.single(threadIdx.x)]), false);
+  if (singles && threadIdx.x < row.singles) run.add_single(to_f32(row.x[row.single(threadIdx.x)]));
   const float target = t >= 0 && t < row.V ? to_f32(row.x[t]) : 0.f;
-  Sums a = merge_block<true, false>(run.sums(), run.c);
+  Sums a = merge_block<true>(run.sums(), run.c);
   if constexpr (TOP) block_top(space, row, v0, v1, singles, most, p.top_k);
   if (C > 1) {
     cluster_wait();  // every block has begun
@@ -604,10 +573,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(LogitsArgs p, 
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    a = merge_lanes<true, false>(peers[threadIdx.x % C], run.c, C);
+    a = merge_lanes<true>(peers[threadIdx.x % C], run.c, C);
     if constexpr (TOP) merge_lists(peer_top, C, p.top_k, space.top);
   }
-  const Stats st = finish<T, true, false>(p, row, a, [](int) { return false; });
+  const Stats st = finish<T, true>(p, row, a);
   if (threadIdx.x == 0) {
     float lp = 0.f;
     if (t != p.ignore_index) {
@@ -752,6 +721,7 @@ struct Teacher {
   float mass;     // sum of the q
   float rest;     // what is left for the other entries (teacher_lse given)
   bool bad;       // an id out of range
+  bool twice;     // an id that is there more than once
 };
 
 __device__ __forceinline__ float teacher_q(const LogitsArgs& p, int id, float logit, float m, float logs, float& lq) {
@@ -769,8 +739,10 @@ struct Entries {
   int id[kPerThread];  // -1: none
   float logit[kPerThread];
   bool bad;            // one of them is out of range
+  float lse;           // the row's teacher_lse, or 0
   __device__ __forceinline__ void read(const LogitsArgs& p, uint32_t r) {
     bad = false;
+    lse = p.teacher_lse ? p.teacher_lse[r] : 0.f;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       const int k = threadIdx.x + i * kThreads;
@@ -786,59 +758,104 @@ struct Entries {
   }
 };
 
-__device__ __forceinline__ float sum_block(float v) {
-  __shared__ float part[kWarps];
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+// The teacher's entries of a row as a set: a table of ids, at most half full.
+constexpr int kSlots = 2 * kMaxEntries;
+struct EntrySet {
+  int slot[kSlots];  // -1: free
+  __device__ __forceinline__ void clear() {
+    for (int i = threadIdx.x; i < kSlots; i += kThreads) slot[i] = -1;
+  }
+  static __device__ __forceinline__ int place(int id) { return (int)((uint32_t)id * 2654435769u >> 23); }
+  // true for one of those that put the same id in
+  __device__ __forceinline__ bool put(int id) {
+    for (int h = place(id);; h = (h + 1) % kSlots) {
+      const int was = atomicCAS(&slot[h], -1, id);
+      if (was < 0 || was == id) return was < 0;
+    }
+  }
+  __device__ __forceinline__ bool holds(int id) const {
+    for (int h = place(id);; h = (h + 1) % kSlots)
+      if (slot[h] < 0 || slot[h] == id) return slot[h] == id;
+  }
+};
+static_assert(kSlots == 1 << (32 - 23), "place() gives a slot");
+
+// Both sums over the block, in every thread; once per N in a kernel.
+template <int N>
+__device__ __forceinline__ float2 sum_block(float2 v) {
+  __shared__ float2 part[kWarps];
+  for (int o = 16; o > 0; o >>= 1) {
+    v.x += __shfl_xor_sync(~0u, v.x, o);
+    v.y += __shfl_xor_sync(~0u, v.y, o);
+  }
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = v;
   __syncthreads();
   v = part[0];
 #pragma unroll
-  for (int i = 1; i < kWarps; ++i) v += part[i];
+  for (int i = 1; i < kWarps; ++i) {
+    v.x += part[i].x;
+    v.y += part[i].y;
+  }
   return v;
 }
 
 // By the whole block.
-__device__ __forceinline__ Teacher teacher_stats(const LogitsArgs& p, uint32_t r, const Entries& e) {
-  __shared__ float part[kWarps];
+__device__ __forceinline__ Teacher teacher_stats(const LogitsArgs& p, const Entries& e, bool twice) {
   Teacher t;
+  t.m = 0.f;
+  t.logs = e.lse;
+  if (!p.teacher_lse) {
+    __shared__ float part[kWarps];
+    float m = -kInf;
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i)
+      if (e.id[i] >= 0) m = fmaxf(m, e.logit[i]);
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) m = fmaxf(m, part[i]);
+    if (m != -kInf) t.m = m;
+  }
+  // sum q; how many threads have an entry, a repeated one (2^8 each), a bad one (2^16 each)
+  float2 s = make_float2(0.f, (twice ? 256.f : 0.f) + (e.bad ? 65536.f : 0.f));
   bool some = false;
-  float m = -kInf;
+  float lq;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i)
-    if (e.id[i] >= 0) {
-      some = true;
-      m = fmaxf(m, e.logit[i]);
-    }
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
-  some = __syncthreads_or(some);
-  t.bad = __syncthreads_or(e.bad);
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, part[i]);
-  t.m = p.teacher_lse || m == -kInf ? 0.f : m;
-  t.logs = p.teacher_lse ? (some ? p.teacher_lse[r] : kInf) : 0.f;
-  float s = 0.f, lq;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) s += teacher_q(p, e.id[i], e.logit[i], t.m, t.logs, lq);
-  s = sum_block(s);
+  for (int i = 0; i < kPerThread; ++i) {
+    some |= e.id[i] >= 0;
+    s.x += teacher_q(p, e.id[i], e.logit[i], t.m, t.logs, lq);
+  }
+  s.y += some;
+  s = sum_block<0>(s);
+  const uint32_t threads = (uint32_t)s.y;
+  some = threads % 256 != 0;
+  t.twice = threads / 256 % 256 != 0;
+  t.bad = threads / 65536 != 0;
   if (p.teacher_lse) {
-    t.mass = s;
-    t.rest = some ? fmaxf(0.f, 1.f - s) : 0.f;
+    if (!some) t.logs = kInf;
+    t.mass = some ? s.x : 0.f;
+    t.rest = some ? fmaxf(0.f, 1.f - s.x) : 0.f;
   } else {
-    t.logs = s == 0.f ? kInf : logf(s);
-    t.mass = s == 0.f ? 0.f : 1.f;
+    t.logs = s.x == 0.f ? kInf : logf(s.x);
+    t.mass = s.x == 0.f ? 0.f : 1.f;
     t.rest = 0.f;
   }
   return t;
 }
 
-// REST: teacher_lse is given, and the sum outside of the entries is needed on
-// its own (1 - sum p_k would cancel): one byte per vector says which of its
-// values are entries.
-template <typename T, bool REST>
+// With teacher_lse, what is left over is one more class: q_r = 1 - Q against
+// p_r = 1 - P, with P the sum of p at the entries, each once. An error d of P
+// is one of d q_r / p_r of the loss, no more than those of its other terms
+// unless the model leaves much less than the teacher; rows where it leaves less
+// than a quarter of q_r are walked once more for p_r itself. (Keeping that sum
+// in the pass, by a byte of marks per vector, took 8 us of the 58 of 4096 x
+// 32000 bf16 with 64 entries.) The ratio q_r / p_r is 1 + (P - Q) / p_r, whose
+// difference keeps its digits where the entries hold little: the quotient is
+// off by up to 2 10^-5 of such a loss, this by 10^-6.
+template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) {
-  extern __shared__ uint32_t marks[];
-  __shared__ uint32_t single_marks;
+  __shared__ EntrySet set;
   __shared__ Sums peers[kMaxCluster];
   griddep_wait();
   const uint32_t r = blockIdx.x / C;
@@ -847,31 +864,26 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   const Row<T> row(p, r);
   const int per = (row.vectors + C - 1) / C;
   const int v0 = min(rank * per, row.vectors), v1 = min(v0 + per, row.vectors);
-  Running<T, false, REST> run(scale_of(p));
-  const uint8_t* mark = reinterpret_cast<const uint8_t*>(marks);
+  Running<T, false> run(scale_of(p));
   Entries entries;
   float given[kPerThread];  // the model's logits there
-  bool fresh[kPerThread];   // the values of this block that are entries, each once
+  bool fresh[kPerThread];   // counted in P
+  Teacher t;
   auto first = [&] {
+    if (rank != 0) return;
     entries.read(p, r);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) given[i] = entries.id[i] >= 0 ? to_f32(row.x[entries.id[i]]) : 0.f;
-    if constexpr (REST) {
-      for (int i = threadIdx.x; i < (v1 - v0 + 3) / 4; i += kThreads) marks[i] = 0;
-      if (threadIdx.x == 0) single_marks = 0;
-      __syncthreads();
+    set.clear();
+    __syncthreads();
+    bool twice = false;
 #pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        const int id = entries.id[i];
-        fresh[i] = false;
-        if (id < 0) continue;
-        const int v = row.place(id);
-        auto claim = [&](uint32_t* word, uint32_t bit) { fresh[i] = !(atomicOr(word, bit) & bit); };
-        if (v >= v0 && v < v1) claim(&marks[(v - v0) / 4], 1u << ((v - v0) % 4 * 8 + (id - row.lead) % Row<T>::E));
-        else if (v < 0 && rank == 0) claim(&single_marks, 1u << (-1 - v));
-      }
-      __syncthreads();
+    for (int i = 0; i < kPerThread; ++i) {
+      fresh[i] = entries.id[i] >= 0 && set.put(entries.id[i]);
+      twice |= entries.id[i] >= 0 && !fresh[i];
     }
+    __syncwarp();  // threads that looked further are waited for here, not all along the row
+    t = teacher_stats(p, entries, twice);
   };
   each_vectors(row, v0, v1, first, [&](const uint4* raw, int v) {
     float top = -kInf;
@@ -879,49 +891,41 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
     for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, Vec<T>::max(raw[u]));
     run.see(top);
 #pragma unroll
-    for (int u = 0; u < kUnroll; ++u) run.add(raw[u], REST && v + u * kThreads < v1 ? mark[v + u * kThreads - v0] : 0);
+    for (int u = 0; u < kUnroll; ++u) run.add(raw[u]);
   });
-  if (rank == 0 && threadIdx.x < row.singles)
-    run.add_single(to_f32(row.x[row.single(threadIdx.x)]), REST && (single_marks >> threadIdx.x & 1));
-  if constexpr (REST)
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) run.see(fresh[i] ? given[i] : -kInf);
-  Sums a = run.sums();
-  if constexpr (REST)
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) a.u += exp2_approx(fmaf(fresh[i] ? given[i] : -kInf, run.c, -run.M));
-  a = merge_block<false, REST>(a, run.c);
+  if (rank == 0 && threadIdx.x < row.singles) run.add_single(to_f32(row.x[row.single(threadIdx.x)]));
+  Sums a = merge_block<false>(run.sums(), run.c);
   if (C > 1) {
     cluster_wait();
     if (threadIdx.x == 0) *in_block(&peers[rank], 0) = a;
     cluster_arrive();
     cluster_wait();
     if (rank != 0) return;
-    a = merge_lanes<false, REST>(peers[threadIdx.x % C], run.c, C);
+    a = merge_lanes<false>(peers[threadIdx.x % C], run.c, C);
   }
-  const Stats st = finish<T, false, REST>(p, row, a, [&](int j) {
-    for (int k = 0; k < p.entries; ++k)
-      if (p.teacher_ids[(int64_t)r * p.entries + k] == j) return true;
-    return false;
-  });
-  const Teacher t = teacher_stats(p, r, entries);
-  float loss = 0.f;
+  const Stats st = finish<T, false>(p, row, a);
+  float2 sums = make_float2(0.f, 0.f);  // of the entries' terms, and of 2^y at them
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     float lq;
     const float q = teacher_q(p, entries.id[i], entries.logit[i], t.m, t.logs, lq);
-    if (q != 0.f) loss += q * (lq - st.logprob(given[i]));
+    if (q != 0.f) sums.x += q * (lq - st.logprob(given[i]));
+    if (fresh[i]) sums.y += exp2_approx(st.y(given[i]));
   }
-  __syncthreads();
-  loss = sum_block(loss);
-  // The rest as a class. With q_r = 1 - Q and p_r = 1 - P the ratio q_r / p_r is
-  // 1 + (P - Q) / p_r, whose difference keeps its digits where the entries hold
-  // little: there a quotient of two rounded sums near 1 is off by 10^-5 of the
-  // loss, this by 10^-7.
+  sums = sum_block<1>(sums);
+  float loss = sums.x;
   float outside = t.mass;  // what p outside of the entries is multiplied by: Q + q_r - q_r / p_r
-  if (REST && t.rest > 0.f) {
-    const float more = st.rest == 0.f ? kInf : (st.in - t.mass) / st.rest;
-    loss += t.rest * (fabsf(more) < 0.5f ? log1pf(more) : logf(t.rest / st.rest));
+  if (t.rest > 0.f) {
+    const float in = st.empty() ? 0.f : sums.y / st.s;
+    float out = st.empty() ? 0.f : 1.f - in;
+    if (4.f * out < t.rest && !st.empty()) {  // the same for every thread
+      float s = 0.f;
+      for (int j = threadIdx.x; j < row.V; j += kThreads)
+        if (!set.holds(j)) s += exp2_approx(st.y(to_f32(row.x[j])));
+      out = sum_block<2>({s, 0.f}).x / st.s;
+    }
+    const float more = out == 0.f ? kInf : (in - t.mass) / out;
+    loss += t.rest * (fabsf(more) < 0.5f ? log1pf(more) : logf(t.rest / out));
     outside = isinf(more) ? 0.f : -more;  // infinite: every p outside is 0
   }
   if (threadIdx.x != 0) return;
@@ -938,12 +942,13 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
     keep[3] = t.logs;
     keep[4] = t.bad ? kNaN : t.mass + t.rest;
     keep[5] = t.bad ? kNaN : outside;
+    keep[6] = t.twice;
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p, int chunks, int span) {
-  __shared__ __align__(16) int id_of[kMaxEntries];
+  __shared__ int id_of[kMaxEntries];
   __shared__ float q_of[kMaxEntries];
   griddep_wait();
   const uint32_t r = blockIdx.x / chunks;
@@ -956,19 +961,22 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   const float g = p.dloss[r] * p.inv_temperature;
   // dlogits_j = p_j outer, or for an entry p_j inner - its q
   const float inner = keep[4] * g, outer = keep[5] * g;
+  const bool twice = keep[6] != 0.f;
   Entries entries;
-  float given[kPerThread];
+  float given[kPerThread], q[kPerThread];
   bool mine[kPerThread];  // this block writes it
   auto first = [&] {
     entries.read(p, r);
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       float lq;
-      const int k = threadIdx.x + i * kThreads;
-      q_of[k] = teacher_q(p, entries.id[i], entries.logit[i], keep[2], keep[3], lq);
-      id_of[k] = entries.id[i];
+      q[i] = teacher_q(p, entries.id[i], entries.logit[i], keep[2], keep[3], lq);
       mine[i] = entries.id[i] >= 0 && writes(row, entries.id[i], chunk, v0, v1);
       given[i] = mine[i] ? to_f32(row.x[entries.id[i]]) : 0.f;
+      if (twice) {
+        q_of[threadIdx.x + i * kThreads] = q[i];
+        id_of[threadIdx.x + i * kThreads] = entries.id[i];
+      }
     }
   };
   auto prob = [&](float x) { return exp2_approx(st.y(x) - st.l2s); };
@@ -992,25 +1000,20 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   if (zero) return;
   __syncthreads();
   // the entries once more, each by the first that names it, with the q of all that do
-  const int4* four = reinterpret_cast<const int4*>(id_of);
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
     if (!mine[i]) continue;
     const int j = entries.id[i], self = threadIdx.x + i * kThreads;
-    float q = 0.f;
     int first = self;
-    auto same = [&](int k) {
-      first = min(first, k);
-      q += q_of[k];
-    };
-    for (int k = 0; 4 * k < p.entries; ++k) {
-      const int4 ids = four[k];
-      if (ids.x == j) same(4 * k);
-      if (ids.y == j) same(4 * k + 1);
-      if (ids.z == j) same(4 * k + 2);
-      if (ids.w == j) same(4 * k + 3);
+    if (twice) {
+      q[i] = 0.f;
+      for (int k = 0; k < p.entries; ++k)
+        if (id_of[k] == j) {
+          first = min(first, k);
+          q[i] += q_of[k];
+        }
     }
-    if (first == self) out[j] = from_f32<T>(prob(given[i]) * inner - q * g);
+    if (first == self) out[j] = from_f32<T>(prob(given[i]) * inner - q[i] * g);
   }
 }
 
@@ -1079,8 +1082,7 @@ cudaError_t launch_token_logprobs_backward(int dtype, const LogitsArgs& p, cudaS
 cudaError_t launch_distill(int dtype, const LogitsArgs& p, cudaStream_t stream) {
   return by_type(dtype, [&](auto t) {
     typedef decltype(t) T;
-    if (p.teacher_lse) return launch_rows(distill_kernel<T, true>, p, Vec<T>::E, 1, stream);
-    return launch_rows(distill_kernel<T, false>, p, Vec<T>::E, 0, stream);
+    return launch_rows(distill_kernel<T>, p, Vec<T>::E, 0, stream);
   });
 }
 
