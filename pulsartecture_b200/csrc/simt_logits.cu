@@ -610,9 +610,10 @@ constexpr int kRound = kUnroll * kThreads;  // vectors of a block's loads in fli
 
 // Writes f(pair of logits) over the block's vectors [v0, v1) of a row, or zeros.
 // Stores are as wide as the loads where both rows lie alike. `first` is done
-// while the first loads are on their way, not with zeros.
-template <typename T, typename G, typename F>
-__device__ __forceinline__ void map_vectors(const Row<T>& row, T* out, int v0, int v1, bool zero, G first, F f) {
+// while the first loads are on their way, not with zeros; `patch` changes a
+// vector's results (given its logits and number) before they are stored.
+template <typename T, typename G, typename F, typename P>
+__device__ __forceinline__ void map_vectors(const Row<T>& row, T* out, int v0, int v1, bool zero, G first, F f, P patch) {
   const bool wide = (((uintptr_t)row.x ^ (uintptr_t)out) & 15) == 0;
   auto put = [&](uint4 got, int v) {
     T* to = out + row.lead + v * Row<T>::E;
@@ -635,7 +636,9 @@ __device__ __forceinline__ void map_vectors(const Row<T>& row, T* out, int v0, i
         uint64_t d[Row<T>::E / 2];
 #pragma unroll
         for (int i = 0; i < Row<T>::E / 2; ++i) d[i] = f(raw[u], i);
-        put(Vec<T>::put(d), v + u * kThreads);
+        uint4 got = Vec<T>::put(d);
+        patch(got, raw[u], v + u * kThreads);
+        put(got, v + u * kThreads);
       }
   });
 }
@@ -686,7 +689,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
         const uint64_t e = sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y)));
         if constexpr (decltype(sloped)::value) return sm100::f2_mul(e, sm100::f2_fma(l, s2, f2));
         else return sm100::f2_mul(e, f2);
-      });
+      }, [](uint4&, const uint4&, int) {});
     };
     if (slope == 0.f) map(std::false_type{});
     else map(std::true_type{});
@@ -849,7 +852,7 @@ __device__ __forceinline__ Teacher teacher_stats(const LogitsArgs& p, const Entr
 // is one of d q_r / p_r of the loss, no more than those of its other terms
 // unless the model leaves much less than the teacher; rows where it leaves less
 // than a quarter of q_r are walked once more for p_r itself. (Keeping that sum
-// in the pass, by a byte of marks per vector, took 8 us of the 58 of 4096 x
+// in the pass, by a byte of marks per vector, took 8 us of the 59 of 4096 x
 // 32000 bf16 with 64 entries.) The ratio q_r / p_r is 1 + (P - Q) / p_r, whose
 // difference keeps its digits where the entries hold little: the quotient is
 // off by up to 2 10^-5 of such a loss, this by 10^-6.
@@ -879,8 +882,10 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
     bool twice = false;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      fresh[i] = entries.id[i] >= 0 && set.put(entries.id[i]);
-      twice |= entries.id[i] >= 0 && !fresh[i];
+      fresh[i] = false;
+      if (entries.id[i] < 0) continue;
+      fresh[i] = set.put(entries.id[i]);
+      twice |= !fresh[i];
     }
     __syncwarp();  // threads that looked further are waited for here, not all along the row
     t = teacher_stats(p, entries, twice);
@@ -946,10 +951,29 @@ __global__ void __launch_bounds__(kThreads) distill_kernel(LogitsArgs p, int C) 
   }
 }
 
+// What a block's entries subtract from their p_j inner, kept by vector: one bit
+// per vector says whether it has an entry (the 32 vectors of a warp share a word),
+// and those that have take one of kMaxEntries cells each.
+template <int E>
+struct Cells {
+  __align__(16) float q[kMaxEntries][E];
+  uint32_t has[kMaxEntries];  // bit e: value e of the cell's vector is an entry
+  uint32_t count;
+  float single_q[2 * E];
+  uint32_t single_has;
+};
+
+// The entries go out with the rest of their vectors. (Writing them once more
+// behind the pass took 10 us more for 64 of them on 4096 x 32000 bf16 and 30
+// us for 256: their lines had left the cache by then.)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p, int chunks, int span) {
+  constexpr int E = Row<T>::E;
+  extern __shared__ uint32_t marks[];  // span / 32 words of bits, then each word's first cell
+  __shared__ Cells<E> cells;
   __shared__ int id_of[kMaxEntries];
   __shared__ float q_of[kMaxEntries];
+  uint8_t* base = reinterpret_cast<uint8_t*>(marks + span / 32);
   griddep_wait();
   const uint32_t r = blockIdx.x / chunks;
   const int chunk = blockIdx.x - r * chunks;
@@ -961,59 +985,102 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   const float g = p.dloss[r] * p.inv_temperature;
   // dlogits_j = p_j outer, or for an entry p_j inner - its q
   const float inner = keep[4] * g, outer = keep[5] * g;
-  const bool twice = keep[6] != 0.f;
-  Entries entries;
-  float given[kPerThread], q[kPerThread];
-  bool mine[kPerThread];  // this block writes it
+  auto cell = [&](int v) { return base[v / 32] + __popc(marks[v / 32] & ((1u << v % 32) - 1)); };
   auto first = [&] {
+    Entries entries;
     entries.read(p, r);
+    const int words = (v1 - v0 + 31) / 32;
+    for (int i = threadIdx.x; i < words; i += kThreads) marks[i] = 0;
+    for (int i = threadIdx.x; i < kMaxEntries; i += kThreads) cells.has[i] = 0;
+    if (threadIdx.x == 0) cells.count = cells.single_has = 0;
+    const bool twice = keep[6] != 0.f;
+    float q[kPerThread];
+    int at[kPerThread];  // its vector in the span, -1 - its single, or none of both
+    constexpr int kNone = INT32_MIN;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
       float lq;
-      q[i] = teacher_q(p, entries.id[i], entries.logit[i], keep[2], keep[3], lq);
-      mine[i] = entries.id[i] >= 0 && writes(row, entries.id[i], chunk, v0, v1);
-      given[i] = mine[i] ? to_f32(row.x[entries.id[i]]) : 0.f;
+      const int j = entries.id[i];
+      q[i] = teacher_q(p, j, entries.logit[i], keep[2], keep[3], lq) * g;
+      at[i] = kNone;
+      if (j >= 0 && writes(row, j, chunk, v0, v1)) at[i] = row.place(j) < 0 ? row.place(j) : row.place(j) - v0;
       if (twice) {
         q_of[threadIdx.x + i * kThreads] = q[i];
-        id_of[threadIdx.x + i * kThreads] = entries.id[i];
+        id_of[threadIdx.x + i * kThreads] = j;
       }
     }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      if (at[i] == kNone) continue;
+      if (twice) {  // the first that names it, with the q of all that do, in their order
+        const int j = entries.id[i], self = threadIdx.x + i * kThreads;
+        int first = self;
+        q[i] = 0.f;
+        for (int k = 0; k < p.entries; ++k)
+          if (id_of[k] == j) {
+            first = min(first, k);
+            q[i] += q_of[k];
+          }
+        if (first != self) {
+          at[i] = kNone;
+          continue;
+        }
+      }
+      if (at[i] >= 0) {
+        atomicOr(&marks[at[i] / 32], 1u << at[i] % 32);
+      } else {
+        atomicOr(&cells.single_has, 1u << (-1 - at[i]));
+        cells.single_q[-1 - at[i]] = q[i];
+      }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < words; i += kThreads)
+      if (const uint32_t word = marks[i]) base[i] = (uint8_t)atomicAdd(&cells.count, __popc(word));
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i)
+      if (at[i] >= 0) {
+        const int c = cell(at[i]), e = (entries.id[i] - row.lead) % E;
+        cells.q[c][e] = q[i];
+        atomicOr(&cells.has[c], 1u << e);
+      }
+    __syncthreads();
   };
   auto prob = [&](float x) { return exp2_approx(st.y(x) - st.l2s); };
   const bool zero = g == 0.f || (st.empty() && !isnan(inner));
   if (st.far) {
-    first();
-    for (int j = row.lead + v0 * Row<T>::E + threadIdx.x; j < row.lead + v1 * Row<T>::E; j += kThreads)
-      out[j] = from_f32<T>(zero ? 0.f : prob(to_f32(row.x[j])) * outer);
+    if (!zero) first();
+    for (int v = v0 + threadIdx.x; v < v1; v += kThreads)
+      for (int e = 0; e < E; ++e) {
+        const int j = row.lead + v * E + e;
+        const float f = zero ? 0.f : prob(to_f32(row.x[j]));
+        const bool marked = !zero && marks[(v - v0) / 32] >> (v - v0) % 32 & 1;
+        const int c = marked ? cell(v - v0) : 0;
+        out[j] = from_f32<T>(marked && cells.has[c] >> e & 1 ? f * inner - cells.q[c][e] : f * outer);
+      }
   } else {
     const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
     const uint64_t o2 = sm100::f2_splat(outer);
     map_vectors(row, out, v0, v1, zero, first, [&](const uint4& raw, int i) {
       const float2 f = sm100::f2_split(sm100::f2_add(sm100::f2_fma(Vec<T>::pair(raw, i), c2, nM), nl));
       return sm100::f2_mul(sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y))), o2);
+    }, [&](uint4& got, const uint4& raw, int v) {
+      if (marks[(v - v0) / 32] >> (v - v0) % 32 & 1) {
+        const int c = cell(v - v0);
+        const uint32_t has = cells.has[c];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float f = prob(to_f32(reinterpret_cast<const T*>(&raw)[e])) * inner - cells.q[c][e];
+          if (has >> e & 1) reinterpret_cast<T*>(&got)[e] = from_f32<T>(f);
+        }
+      }
     });
   }
   if (chunk == 0 && threadIdx.x < row.singles) {
     const int j = row.single(threadIdx.x);
-    out[j] = from_f32<T>(zero ? 0.f : prob(to_f32(row.x[j])) * outer);
-  }
-  if (zero) return;
-  __syncthreads();
-  // the entries once more, each by the first that names it, with the q of all that do
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    if (!mine[i]) continue;
-    const int j = entries.id[i], self = threadIdx.x + i * kThreads;
-    int first = self;
-    if (twice) {
-      q[i] = 0.f;
-      for (int k = 0; k < p.entries; ++k)
-        if (id_of[k] == j) {
-          first = min(first, k);
-          q[i] += q_of[k];
-        }
-    }
-    if (first == self) out[j] = from_f32<T>(prob(given[i]) * inner - q[i] * g);
+    const float f = zero ? 0.f : prob(to_f32(row.x[j]));
+    out[j] = from_f32<T>(!zero && cells.single_has >> threadIdx.x & 1 ? f * inner - cells.single_q[threadIdx.x] : f * outer);
   }
 }
 
@@ -1047,15 +1114,17 @@ cudaError_t launch_rows(K kernel, const LogitsArgs& p, int per_vector, int bytes
 }
 
 // A row's gradient is split into spans of whole rounds of loads, as long as
-// every SM still gets kBlocks blocks.
+// every SM still gets kBlocks blocks. `marks`: 5 bytes of shared memory per 32
+// vectors (a span is at most 2^20 / 4 vectors: 40 KB, and 8 KB beside them).
 template <typename K>
-cudaError_t launch_spans(K kernel, const LogitsArgs& p, int per_vector, cudaStream_t stream) {
+cudaError_t launch_spans(K kernel, const LogitsArgs& p, int per_vector, bool marks, cudaStream_t stream) {
   const int64_t rows = p.batch * p.rows, rounds = (p.vocab / per_vector + kRound - 1) / kRound;
   int64_t chunks = (kBlocks * fakla_sm_count() + rows - 1) / rows;
   if (chunks > rounds) chunks = rounds;
   if (chunks < 1) chunks = 1;
   const int span = (int)((rounds + chunks - 1) / chunks) * kRound;
-  return launch_chained(kernel, dim3((unsigned)(rows * chunks)), dim3(kThreads), 0, stream, 1u, p, (int)chunks, span);
+  return launch_chained(kernel, dim3((unsigned)(rows * chunks)), dim3(kThreads),
+                        marks ? (size_t)span / 32 * 5 : 0, stream, 1u, p, (int)chunks, span);
 }
 
 template <typename F>
@@ -1075,7 +1144,7 @@ cudaError_t launch_token_logprobs(int dtype, const LogitsArgs& p, cudaStream_t s
 
 cudaError_t launch_token_logprobs_backward(int dtype, const LogitsArgs& p, cudaStream_t stream) {
   return by_type(dtype, [&](auto t) {
-    return launch_spans(token_logprobs_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
+    return launch_spans(token_logprobs_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, false, stream);
   });
 }
 
@@ -1088,7 +1157,7 @@ cudaError_t launch_distill(int dtype, const LogitsArgs& p, cudaStream_t stream) 
 
 cudaError_t launch_distill_backward(int dtype, const LogitsArgs& p, cudaStream_t stream) {
   return by_type(dtype, [&](auto t) {
-    return launch_spans(distill_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, stream);
+    return launch_spans(distill_backward_kernel<decltype(t)>, p, Vec<decltype(t)>::E, true, stream);
   });
 }
 

@@ -412,6 +412,50 @@ def test_distill_small_divergences(cuda, rows, V, dtype):
     _within(got[:, rest], want["dlogits"][:, rest], off[:, rest] / T, "dlogits")
 
 
+@pytest.mark.parametrize("V", [259, 4099, 40001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_distill_neighbouring_entries(cuda, V, dtype):
+    """256 entries side by side, at a row's start, at its end and in between:
+    vectors of nothing but entries, and rows that start on no vector."""
+    rows, K = 6, 256
+    full = torch.randn(rows, V, generator=torch.Generator().manual_seed(V)) * 2
+    at = torch.tensor([0, V - K, (V - K) // 2, 0, V - K, (V - K) // 3])
+    ids = at[:, None] + torch.arange(K)
+    ids[3:] = ids[3:].flip(-1)
+    ids[2, 7] = ids[2, 200]
+    lse = torch.logsumexp(full, -1)
+    logits = (full + 0.5 * torch.randn(rows, V, generator=torch.Generator().manual_seed(1))).to(dtype)
+    _check_distill(cuda, logits, ids, full.gather(-1, ids), None, 1.0)
+    _check_distill(cuda, logits, ids, full.gather(-1, ids), lse + 0.7, 1.0)
+
+
+@pytest.mark.parametrize("rows,V", [(3, 40001), (200, 1000)])
+@pytest.mark.parametrize("scale", [1.5, 3.0, 8.0, 1e6])
+def test_distill_model_sharper_than_the_teacher(cuda, rows, V, scale):
+    """The model leaves less than the teacher outside of the entries: a little,
+    much (its sum is then taken on its own), nothing."""
+    ids, top, lse, full = _teacher((rows,), V, 40, 5, 1.0)
+    _check_distill(cuda, full * scale, ids, top, lse, 1.0, grads=scale < 1e6)
+
+
+def test_distill_largest_vocabulary(cuda):
+    """One block to a row of 2^20 fp32 logits in the backward: the most shared memory."""
+    from pulsartecture_b200 import distill_topk
+
+    rows, V = 600, 1 << 20
+    leaf = torch.zeros(rows, V, device=cuda).requires_grad_()
+    ids = torch.tensor([[5, V - 1, V // 2, V // 2]], device=cuda).expand(rows, 4)
+    loss = distill_topk(leaf, ids, torch.zeros(rows, 4, device=cuda))
+    # q = 1/4 each: log(1/4) - log(1/V); sums of equal powers of two are exact
+    _within(loss, torch.tensor(18 * math.log(2.0)).double(), torch.tensor(16 * U * 13), "loss")
+    g, = torch.autograd.grad(loss.sum(), leaf)
+    want = torch.full((V,), 2.0 ** -20, dtype=torch.float64)
+    want[[5, V - 1]] -= 0.25
+    want[V // 2] -= 0.5
+    for r in (0, 333, rows - 1):
+        _within(g[r], want, 16 * U * want.abs(), "dlogits")
+
+
 def test_distill_rows_without_a_distribution(cuda):
     from pulsartecture_b200 import _lib, distill_topk
     from pulsartecture_b200.backend.interface import device_status
