@@ -473,7 +473,8 @@ int fakla_token_logprobs(const void* logits, const int64_t* targets, float* logp
  *   dlogits_j = (w (1[j = target] - p_j) - dentropy p_j (log p_j + entropy)
  *                + sum_k dtop_k (1[j = top_ids_k] - p_j)) / temperature
  * with w = dlogprobs, 0 where the target is ignored. A row of nothing but
- * -inf gets 0; one with a NaN, a +inf or a bad target gets NaN.
+ * -inf, or given only zeros, gets 0; another with a NaN or +inf, and one with a
+ * bad target, gets NaN.
  *
  * Reference: none.
  *   targets, entropy, top_ids, stats : as given to and written by the forward

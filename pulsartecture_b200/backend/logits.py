@@ -133,7 +133,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, top_k: int = 
         empty = logits.new_empty(lead, dtype=torch.float32) + 0 * logits.sum()
         top = ids = None
         if top_k:
-            top, ids = logits.new_empty(*lead, top_k, dtype=torch.float32), targets.new_empty(*lead, top_k)
+            top, ids = empty[..., None].repeat_interleave(top_k, -1), targets.new_empty(*lead, top_k)
         return TokenLogprobs(empty, empty.clone(), top, ids)
     targets = targets.contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:

@@ -117,11 +117,11 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor
     dev, code, act = _check_gated(x, gate, state, gate_act, 3)
     mix = bool(mix)
     if x.numel() == 0:
-        B, T, D = x.shape
+        B, _, D = x.shape
         final = None
         if return_state:
             final = state.clone() if state is not None else torch.zeros(B, D, device=dev, dtype=torch.float32)
-        return torch.empty(B, T, D, device=dev, dtype=x.dtype), final
+        return x * gate, final  # nothing, but with x and gate behind it
     x, gate = _dense_channels(x), _dense_channels(gate)
     state = None if state is None else state.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or

@@ -250,6 +250,18 @@ def test_no_tokens(cuda):
     assert out.shape == (0, 5)
 
 
+@pytest.mark.parametrize("shape", [(2, 0, 5), (0, 3, 5), (2, 3, 0)])
+def test_gradients_of_nothing(cuda, shape):
+    from pulsartecture_b200 import gated_scan
+
+    x, gate = torch.empty(shape, device=cuda, requires_grad=True), torch.empty(shape, device=cuda, requires_grad=True)
+    s = torch.randn(shape[0], shape[2], device=cuda, requires_grad=True)
+    out, end = gated_scan(x, gate, s)
+    assert out.shape == shape and out.is_contiguous()
+    (out.sum() + end.sum()).backward()
+    assert x.grad.shape == shape and gate.grad.shape == shape and torch.equal(s.grad, torch.ones_like(s))
+
+
 def test_offsets_past_32_bits(cuda):
     """A batch stride of more than 2^31 elements."""
     from pulsartecture_b200 import gated_scan

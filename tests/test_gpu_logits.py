@@ -572,6 +572,16 @@ def test_no_rows(cuda):
     loss.sum().backward()
 
 
+def test_gradient_of_no_alternatives(cuda):
+    from pulsartecture_b200 import token_logprobs
+
+    logits = torch.empty(0, 50, device=cuda, requires_grad=True)
+    r = token_logprobs(logits, torch.empty(0, dtype=torch.int64, device=cuda), top_k=3)
+    assert r.top_logprobs.shape == (0, 3)
+    r.top_logprobs.sum().backward()
+    assert logits.grad.shape == (0, 50)
+
+
 def test_refusals_on_device_tensors(cuda):
     from pulsartecture_b200 import distill_topk, token_logprobs
 
