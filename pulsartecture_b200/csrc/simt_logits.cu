@@ -1058,7 +1058,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
         const float f = zero ? 0.f : prob(to_f32(row.x[j]));
         const bool marked = !zero && marks[(v - v0) / 32] >> (v - v0) % 32 & 1;
         const int c = marked ? cell(v - v0) : 0;
-        out[j] = from_f32<T>(marked && cells.has[c] >> e & 1 ? f * inner - cells.q[c][e] : f * outer);
+        out[j] = from_f32<T>(zero ? 0.f : marked && cells.has[c] >> e & 1 ? f * inner - cells.q[c][e] : f * outer);
       }
   } else {
     const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
@@ -1081,7 +1081,8 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   if (chunk == 0 && threadIdx.x < row.singles) {
     const int j = row.single(threadIdx.x);
     const float f = zero ? 0.f : prob(to_f32(row.x[j]));
-    out[j] = from_f32<T>(!zero && cells.single_has >> threadIdx.x & 1 ? f * inner - cells.single_q[threadIdx.x] : f * outer);
+    const bool given = !zero && cells.single_has >> threadIdx.x & 1;
+    out[j] = from_f32<T>(zero ? 0.f : given ? f * inner - cells.single_q[threadIdx.x] : f * outer);
   }
 }
 

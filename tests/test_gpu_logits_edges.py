@@ -1,0 +1,51 @@
+"""Rows of logits at the edges of their definition: rows that are given
+nothing, rows without a distribution behind them, a model that leaves next to
+nothing outside of the teacher's entries, temperatures close to 0, repeated
+entries, calls from two threads.
+
+Bounds as in test_gpu_logits.py, u = 2^-24 (GPU only).
+"""
+import threading
+
+import pytest
+import torch
+
+from tests.test_gpu_logits import INF, U, _check_token, _logits, _sum_error, _teacher, _within
+
+pytestmark = pytest.mark.gpu
+
+NAN = float("nan")
+TYPES = [torch.float32, torch.bfloat16]
+# 5003 values: rows start and end on no 16 bytes, in either type
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_rows_given_zero(cuda, dtype, rest):
+    """A row whose loss counts for nothing gets no gradient whatever it holds:
+    a bad id, a NaN or +inf, nothing but -inf, values far from 0."""
+    from pulsartecture_b200 import _lib, distill_topk
+    from pulsartecture_b200.backend.interface import device_status
+
+    device_status()
+    for V in (5003, 40001):
+        rows, K = 14, 6
+        ids, top, lse, full = _teacher((rows,), V, K, V, 1.0)
+        logits = full.to(dtype)
+        ids[0:2, 2] = V
+        ids[2:4, 1] = -100
+        logits[4:6, 7] = NAN
+        logits[6:8, 9] = INF
+        logits[8:10] = -INF
+        logits[10:12] += 3e6  # past where the kernels form their exponents by one product
+        ids[11, 3] = V + 5
+        given = torch.zeros(rows)
+        given[12:] = 1.5
+        leaf = logits.to(cuda).requires_grad_()
+        loss = distill_topk(leaf, ids.to(cuda), top.to(cuda), lse.to(cuda) if rest else None)
+        assert torch.isnan(loss[[0, 1, 2, 3, 4, 5, 6, 7, 11]]).all() and (loss[8:10] == INF).all()
+        g, = torch.autograd.grad(loss, leaf, given.to(cuda))
+        assert not torch.isnan(g).any() and not g[:12].any()
+        assert torch.isfinite(g[12:]).all() and g[12:].any()
+        with pytest.raises(_lib.FaklaError):
+            device_status()
