@@ -524,8 +524,8 @@ int fakla_distill_topk(const void* logits, const int64_t* teacher_ids, const flo
  * with Q = sum_k q_k and S the set of the i_k:
  *   dlogits_j = dloss / temperature * (p_j (Q + q_r) - sum_{k: i_k = j} q_k
  *               - 1[j not in S] q_r p_j / p_r)
- * A row whose dloss is 0 gets 0. Of the others, one with a bad id, a NaN or +inf
- * gets NaN and one of nothing but -inf gets 0.
+ * A row whose dloss is 0, or without an entry (as above), gets 0. Of the others,
+ * one with a bad id, a NaN or +inf gets NaN and one of nothing but -inf gets 0.
  *
  * Reference: none.
  *   stats : written by the forward     dloss : (batch, rows)

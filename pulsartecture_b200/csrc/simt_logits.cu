@@ -1049,7 +1049,9 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
     __syncthreads();
   };
   auto prob = [&](float x) { return exp2_approx(st.y(x) - st.l2s); };
-  const bool zero = g == 0.f || (st.empty() && !isnan(inner));
+  // given nothing, by the loss or by the teacher (Q + q_r is 0 in a row without
+  // entries only), and rows of nothing but -inf
+  const bool zero = g == 0.f || keep[4] == 0.f || (st.empty() && !isnan(inner));
   if (st.far) {
     if (!zero) first();
     for (int v = v0 + threadIdx.x; v < v1; v += kThreads)

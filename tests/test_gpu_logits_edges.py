@@ -49,3 +49,26 @@ def test_distill_rows_given_zero(cuda, dtype, rest):
         assert torch.isfinite(g[12:]).all() and g[12:].any()
         with pytest.raises(_lib.FaklaError):
             device_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rest", [False, True])
+def test_distill_rows_without_entries(cuda, dtype, rest):
+    """No entry: loss 0 and no gradient, whatever the row's logits are."""
+    from pulsartecture_b200 import distill_topk
+
+    for V in (5003, 40001):
+        rows, K = 7, 6
+        ids, top, lse, full = _teacher((rows,), V, K, V, 1.0)
+        logits = full.to(dtype)
+        logits[0, 7] = logits[1, V - 1] = NAN
+        logits[2, 0] = INF
+        logits[3] = -INF
+        logits[4] = -3e6
+        ids[:6] = -1
+        top[5] = NAN  # nothing is read where there is no entry
+        leaf = logits.to(cuda).requires_grad_()
+        loss = distill_topk(leaf, ids.to(cuda), top.to(cuda), lse.to(cuda) if rest else None)
+        g, = torch.autograd.grad(loss.sum(), leaf)
+        assert not loss[:6].any() and not torch.isnan(loss).any() and loss[6] != 0
+        assert not torch.isnan(g).any() and not g[:6].any() and g[6].any()
