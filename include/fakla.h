@@ -474,7 +474,7 @@ int fakla_token_logprobs(const void* logits, const int64_t* targets, float* logp
  *                + sum_k dtop_k (1[j = top_ids_k] - p_j)) / temperature
  * with w = dlogprobs, 0 where the target is ignored. A row of nothing but
  * -inf, or given only zeros, gets 0; another with a NaN or +inf, and one with a
- * bad target, gets NaN.
+ * bad target whose w is not 0, gets NaN.
  *
  * Reference: none.
  *   targets, entropy, top_ids, stats : as given to and written by the forward

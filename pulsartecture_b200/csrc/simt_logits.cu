@@ -662,17 +662,24 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
   const int64_t t = p.targets[r];
   const bool counted = t != p.ignore_index, good = t >= 0 && t < row.V;
   float w = counted && p.dlogprobs ? p.dlogprobs[r] : 0.f;
-  if (counted && !good) w = kNaN;
+  if (w != 0.f && !good) w = kNaN;
   const float h = p.dentropy ? p.dentropy[r] : 0.f;
   float total = w;
-  for (int k = 0; k < p.top_k; ++k) total += p.dtop_logprobs[(int64_t)r * p.top_k + k];
+  bool given = w != 0.f || h != 0.f;
+  for (int k = 0; k < p.top_k; ++k) {
+    const float d = p.dtop_logprobs[(int64_t)r * p.top_k + k];
+    total += d;
+    given |= d != 0.f;
+  }
   // dlogits_j = p_j (flat + slope log2 p_j), and what is given to j itself
-  const float flat = -(total + h * p.entropy[r]) * p.inv_temperature, slope = -h * kLn2 * p.inv_temperature;
+  const float flat = -(total + (h == 0.f ? 0.f : h * p.entropy[r])) * p.inv_temperature;
+  const float slope = -h * kLn2 * p.inv_temperature;
   auto value = [&](float x) {
     const float l = fmaxf(st.y(x) - st.l2s, -1e30f), e = exp2_approx(st.y(x) - st.l2s);
     return e * fmaf(l, slope, flat);
   };
-  bool zero = st.empty() || (flat == 0.f && slope == 0.f);
+  // a row that is given nothing gets 0 even where its p are NaN
+  const bool zero = st.empty() || !given;
   if (st.far) {
     for (int j = row.lead + v0 * Row<T>::E + threadIdx.x; j < row.lead + v1 * Row<T>::E; j += kThreads)
       out[j] = from_f32<T>(zero ? 0.f : value(to_f32(row.x[j])));
@@ -698,7 +705,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
     const int j = row.single(threadIdx.x);
     out[j] = from_f32<T>(zero ? 0.f : value(to_f32(row.x[j])));
   }
-  if (st.empty()) return;
+  if (zero) return;
   __syncthreads();
   // the target and the alternatives once more, with their own gradients
   if (threadIdx.x < p.top_k) {

@@ -72,3 +72,44 @@ def test_distill_rows_without_entries(cuda, dtype, rest):
         g, = torch.autograd.grad(loss.sum(), leaf)
         assert not loss[:6].any() and not torch.isnan(loss).any() and loss[6] != 0
         assert not torch.isnan(g).any() and not g[:6].any() and g[6].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("top_k", [0, 3])
+def test_token_rows_given_zero(cuda, dtype, top_k):
+    """A row that is given only zeros (an ignored target's log probability
+    counts as that) gets no gradient: one with a NaN, one with +inf, one with a
+    target outside of the vocabulary. Given anything, it gets NaN."""
+    from pulsartecture_b200 import _lib, token_logprobs
+    from pulsartecture_b200.backend.interface import device_status
+
+    device_status()
+    for V in (5003, 40001):
+        logits = _logits((12,), V, dtype)
+        logits[0:3, 11] = NAN
+        logits[3:6, V - 1] = INF
+        targets = torch.full((12,), 5)
+        targets[1] = targets[4] = -100
+        targets[6:8] = V
+        given = torch.zeros(12)
+        given[1] = given[4] = 2.0  # ignored
+        given[2] = given[5] = given[7] = given[10] = 2.0
+        leaf = logits.to(cuda).requires_grad_()
+        r = token_logprobs(leaf, targets.to(cuda), top_k=top_k)
+        zeros = torch.zeros(12, device=cuda)
+        for outs, grads in (([r.logprobs], [given]), ([r.logprobs, r.entropy], [given, zeros]),
+                            ([r.logprobs, r.entropy, r.top_logprobs], [given, zeros, torch.zeros(12, top_k)])):
+            if outs[-1] is None:
+                continue
+            g, = torch.autograd.grad(outs, leaf, [t.to(cuda) for t in grads], retain_graph=True)
+            nan = torch.isnan(g)
+            for row in (2, 5, 7):
+                assert nan[row].all(), row
+            for row in (0, 1, 3, 4, 6, 8, 9, 11):
+                assert not nan[row].any() and not g[row].any(), row
+            assert torch.isfinite(g[10]).all() and g[10].any()
+        # the entropy's gradient does not depend on the target
+        g, = torch.autograd.grad(r.entropy, leaf, torch.ones(12, device=cuda))
+        assert torch.isnan(g).any(1).tolist() == [True] * 6 + [False] * 6 and g[6].any()
+        with pytest.raises(_lib.FaklaError):
+            device_status()
