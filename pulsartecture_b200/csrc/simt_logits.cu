@@ -674,9 +674,12 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
   // dlogits_j = p_j (flat + slope log2 p_j), and what is given to j itself
   const float flat = -(total + (h == 0.f ? 0.f : h * p.entropy[r])) * p.inv_temperature;
   const float slope = -h * kLn2 * p.inv_temperature;
+  // 2^l is 0 from kNone down, whose product with the slope (up to 10^30 times
+  // what is given, at the lowest temperature) is finite
+  constexpr float kNone = -200.f;
   auto value = [&](float x) {
-    const float l = fmaxf(st.y(x) - st.l2s, -1e30f), e = exp2_approx(st.y(x) - st.l2s);
-    return e * fmaf(l, slope, flat);
+    const float l = st.y(x) - st.l2s;
+    return exp2_approx(l) * fmaf(fmaxf(l, kNone), slope, flat);
   };
   // a row that is given nothing gets 0 even where its p are NaN
   const bool zero = st.empty() || !given;
@@ -686,7 +689,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_backward_kernel(Logit
   } else {
     const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
     const uint64_t f2 = sm100::f2_splat(flat), s2 = sm100::f2_splat(slope);
-    const float low = -kFar / st.c;
+    const float low = (st.M + kNone) / st.c;
     auto map = [&](auto sloped) {
       map_vectors(row, out, v0, v1, zero, [] {}, [&](const uint4& raw, int i) {
         uint4 v = raw;

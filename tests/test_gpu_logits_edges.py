@@ -113,3 +113,23 @@ def test_token_rows_given_zero(cuda, dtype, top_k):
         assert torch.isnan(g).any(1).tolist() == [True] * 6 + [False] * 6 and g[6].any()
         with pytest.raises(_lib.FaklaError):
             device_status()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1e-30, 1e-9, 1e-4, 1e30])
+def test_extreme_temperatures(cuda, dtype, temperature):
+    """All three gradients where softmax is a maximum, or flat; masked places
+    get 0. Some rows have two largest values, some their maximum at 0."""
+    V = 5003
+    logits = _logits((6,), V, dtype)
+    logits[1, ::3] = -INF
+    logits[2, 1::2] = -INF
+    top = logits[2].max() + 1
+    logits[2, [0, 4000]] = top
+    logits[3] -= logits[3].max()
+    logits[4] -= logits[4].max()
+    logits[4, 2500:] = -INF
+    logits[5, :] = -INF
+    logits[5, V - 1] = 1.0
+    targets = torch.tensor([7, 0, 4000, 5, 3000, V - 1])
+    _check_token(cuda, logits, targets, 2, temperature)
