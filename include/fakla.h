@@ -510,9 +510,9 @@ int fakla_token_logprobs_backward(const void* logits, const int64_t* targets, co
  *   teacher_lse : (batch, rows) or NULL      loss : (batch, rows) fp32, written
  *   stats : (batch, rows, 8) fp32 that the backward reads, or NULL
  * entries <= 256, vocab <= 2^20. A row without an entry (or, without
- * teacher_lse, with none above -inf) gives 0. Entries of the same id count
- * each. An id below -1 or >= vocab gives NaN and sets the device status
- * (FAKLA_ERR_INVALID_ARG).
+ * teacher_lse, with none above -inf) gives 0. A p_r below 2^-10^6 counts as 0 and
+ * gives +inf. Entries of the same id count each. An id below -1 or >= vocab gives
+ * NaN and sets the device status (FAKLA_ERR_INVALID_ARG).
  */
 int fakla_distill_topk(const void* logits, const int64_t* teacher_ids, const float* teacher_logits,
                        const float* teacher_lse, float* loss, float* stats, int64_t batch,

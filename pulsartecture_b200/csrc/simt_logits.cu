@@ -857,13 +857,53 @@ __device__ __forceinline__ Teacher teacher_stats(const LogitsArgs& p, const Entr
   return t;
 }
 
+// The logits that are no entries, of a row without NaN or +inf: the largest and
+// the sum of e^{(x - m) / temperature}. By the whole block.
+struct Outside {
+  float m, s;
+};
+template <typename T>
+__device__ __forceinline__ Outside sum_outside(const Row<T>& row, const EntrySet& set, const Stats& st) {
+  __shared__ float part[kWarps];
+  Outside r = {-kInf, 0.f};
+  for (int j0 = threadIdx.x; j0 < row.V; j0 += kUnroll * kThreads) {
+    float x[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int j = j0 + u * kThreads;
+      x[u] = j < row.V ? to_f32(row.x[j]) : -kInf;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const float y = (x[u] - r.m) * st.c;
+      if (x[u] == -kInf || y < -150.f || set.holds(j0 + u * kThreads)) continue;
+      if (x[u] > r.m) {
+        r.s = fmaf(r.s, exp2_approx(-y), 1.f);
+        r.m = x[u];
+      } else {
+        r.s += exp2_approx(y);
+      }
+    }
+  }
+  float m = r.m;
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) m = fmaxf(m, part[i]);
+  return {m, sum_block<2>({r.m == -kInf ? 0.f : r.s * exp2_approx((r.m - m) * st.c), 0.f}).x};
+}
+
 // With teacher_lse, what is left over is one more class: q_r = 1 - Q against
 // p_r = 1 - P, with P the sum of p at the entries, each once. An error d of P
 // is one of d q_r / p_r of the loss, no more than those of its other terms
 // unless the model leaves much less than the teacher; rows where it leaves less
-// than a quarter of q_r are walked once more for p_r itself. (Keeping that sum
-// in the pass, by a byte of marks per vector, took 8 us of the 59 of 4096 x
-// 32000 bf16 with 64 entries.) The ratio q_r / p_r is 1 + (P - Q) / p_r, whose
+// than a quarter of q_r are walked once more for p_r itself, from the largest
+// logit outside: p_r may be far below the smallest fp32 number, where its
+// logarithm and the p / p_r of the gradient still are ordinary ones. Below
+// 2^-10^6 it counts as 0 (masks of a type's lowest value). (Keeping
+// that sum in the pass, by a byte of marks per vector, took 8 us of the 59 of
+// 4096 x 32000 bf16 with 64 entries.) The ratio q_r / p_r is 1 + (P - Q) / p_r, whose
 // difference keeps its digits where the entries hold little: the quotient is
 // off by up to 2 10^-5 of such a loss, this by 10^-6. Twelve blocks on an SM (40
 // registers a thread) take 49 us for 4096 x 32000 bf16, nine of 56 registers 51.
@@ -931,18 +971,25 @@ __global__ void __launch_bounds__(kThreads, 12) distill_kernel(LogitsArgs p, int
   sums = sum_block<1>(sums);
   float loss = sums.x;
   float outside = t.mass;  // what p outside of the entries is multiplied by: Q + q_r - q_r / p_r
+  Outside rest = {-kInf, 0.f};
   if (t.rest > 0.f) {
-    const float in = st.empty() ? 0.f : sums.y / st.s;
-    float out = st.empty() ? 0.f : 1.f - in;
+    const float in = st.empty() ? 0.f : sums.y / st.s, out = st.empty() ? 0.f : 1.f - in;
     if (4.f * out < t.rest && !st.empty()) {  // the same for every thread
-      float s = 0.f;
-      for (int j = threadIdx.x; j < row.V; j += kThreads)
-        if (!set.holds(j)) s += exp2_approx(st.y(to_f32(row.x[j])));
-      out = sum_block<2>({s, 0.f}).x / st.s;
+      rest = sum_outside(row, set, st);
+      const float lpr = rest.m == -kInf ? -kInf : st.logprob(rest.m) + logf(rest.s);
+      if (lpr >= -kLn2 * kFar) {
+        loss += t.rest * (logf(t.rest) - lpr);
+        outside = expf(lpr) * (t.mass + t.rest) - t.rest;  // of p / p_r
+      } else {  // masked
+        rest.m = -kInf;
+        loss = kInf;
+        outside = 0.f;
+      }
+    } else {
+      const float more = out == 0.f ? kInf : (in - t.mass) / out;
+      loss += t.rest * (fabsf(more) < 0.5f ? log1pf(more) : logf(t.rest / out));
+      outside = isinf(more) ? 0.f : -more;  // infinite: every p outside is 0
     }
-    const float more = out == 0.f ? kInf : (in - t.mass) / out;
-    loss += t.rest * (fabsf(more) < 0.5f ? log1pf(more) : logf(t.rest / out));
-    outside = isinf(more) ? 0.f : -more;  // infinite: every p outside is 0
   }
   if (threadIdx.x != 0) return;
   if (t.bad) {
@@ -959,6 +1006,8 @@ __global__ void __launch_bounds__(kThreads, 12) distill_kernel(LogitsArgs p, int
     keep[4] = t.bad ? kNaN : t.mass + t.rest;
     keep[5] = t.bad ? kNaN : outside;
     keep[6] = t.twice;
+    keep[7] = rest.m;  // -inf: p outside goes by the row's own maximum and sum
+    if (rest.m != -kInf) keep[2] = log2f(rest.s) + stats_of(p, rest.m, 0.f).y(rest.m);  // (t.m is 0 with teacher_lse)
   }
 }
 
@@ -993,8 +1042,12 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   T* out = (T*)p.dlogits + (int64_t)r * p.vocab;
   const float* keep = p.stats + (int64_t)r * kDistillStats;
   const Stats st = stats_of(p, keep[0], keep[1]);
+  const bool apart = keep[7] != -kInf;  // p_r was summed on its own
+  const Stats other = apart ? stats_of(p, keep[7], keep[2]) : st;
+  const float teacher_m = apart ? 0.f : keep[2];
   const float g = p.dloss[r] * p.inv_temperature;
-  // dlogits_j = p_j outer, or for an entry p_j inner - its q
+  // dlogits_j = p_j inner - its q for an entry; otherwise p_j outer or (apart)
+  // p_j / p_r outer, in both cases 2^{y - log2 s} of `other`
   const float inner = keep[4] * g, outer = keep[5] * g;
   auto cell = [&](int v) { return base[v / 32] + __popc(marks[v / 32] & ((1u << v % 32) - 1)); };
   auto first = [&] {
@@ -1012,7 +1065,7 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
     for (int i = 0; i < kPerThread; ++i) {
       float lq;
       const int j = entries.id[i];
-      q[i] = teacher_q(p, j, entries.logit[i], keep[2], keep[3], lq) * g;
+      q[i] = teacher_q(p, j, entries.logit[i], teacher_m, keep[3], lq) * g;
       at[i] = kNone;
       if (j >= 0 && writes(row, j, chunk, v0, v1)) at[i] = row.place(j) < 0 ? row.place(j) : row.place(j) - v0;
       if (twice) {
@@ -1062,19 +1115,22 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   // given nothing, by the loss or by the teacher (Q + q_r is 0 in a row without
   // entries only), and rows of nothing but -inf
   const bool zero = g == 0.f || keep[4] == 0.f || (st.empty() && !isnan(inner));
-  if (st.far) {
+  auto prob_out = [&](float x) { return exp2_approx(other.y(x) - other.l2s); };
+  if (st.far || other.far) {
     if (!zero) first();
     for (int v = v0 + threadIdx.x; v < v1; v += kThreads)
       for (int e = 0; e < E; ++e) {
         const int j = row.lead + v * E + e;
-        const float f = zero ? 0.f : prob(to_f32(row.x[j]));
+        const float x = zero ? 0.f : to_f32(row.x[j]);
         const bool marked = !zero && marks[(v - v0) / 32] >> (v - v0) % 32 & 1;
         const int c = marked ? cell(v - v0) : 0;
-        out[j] = from_f32<T>(zero ? 0.f : marked && cells.has[c] >> e & 1 ? f * inner - cells.q[c][e] : f * outer);
+        const bool given = marked && cells.has[c] >> e & 1;
+        out[j] = from_f32<T>(zero ? 0.f : given ? prob(x) * inner - cells.q[c][e] : prob_out(x) * outer);
       }
   } else {
-    const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-st.M), nl = sm100::f2_splat(-st.l2s);
+    const uint64_t c2 = sm100::f2_splat(st.c), nM = sm100::f2_splat(-other.M), nl = sm100::f2_splat(-other.l2s);
     const uint64_t o2 = sm100::f2_splat(outer);
+    // (an entry's own place is patched, whatever 2^{y - log2 s} of `other` is there)
     map_vectors(row, out, v0, v1, zero, first, [&](const uint4& raw, int i) {
       const float2 f = sm100::f2_split(sm100::f2_add(sm100::f2_fma(Vec<T>::pair(raw, i), c2, nM), nl));
       return sm100::f2_mul(sm100::f2_make(__float_as_uint(exp2_approx(f.x)), __float_as_uint(exp2_approx(f.y))), o2);
@@ -1092,9 +1148,9 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
   }
   if (chunk == 0 && threadIdx.x < row.singles) {
     const int j = row.single(threadIdx.x);
-    const float f = zero ? 0.f : prob(to_f32(row.x[j]));
+    const float x = zero ? 0.f : to_f32(row.x[j]);
     const bool given = !zero && cells.single_has >> threadIdx.x & 1;
-    out[j] = from_f32<T>(zero ? 0.f : given ? f * inner - cells.single_q[threadIdx.x] : f * outer);
+    out[j] = from_f32<T>(zero ? 0.f : given ? prob(x) * inner - cells.single_q[threadIdx.x] : prob_out(x) * outer);
   }
 }
 

@@ -133,3 +133,104 @@ def test_extreme_temperatures(cuda, dtype, temperature):
     logits[5, V - 1] = 1.0
     targets = torch.tensor([7, 0, 4000, 5, 3000, V - 1])
     _check_token(cuda, logits, targets, 2, temperature)
+
+
+def _check_rest(cuda, logits, ids, teacher, lse, temperature):
+    """Loss and gradient with the rest as a class, in logarithms throughout.
+
+    Outside of the entries a gradient is p_j (Q + q_r) - q_r p_j / p_r. Both
+    terms go by their own size: p_j is off by 8 u of its logarithm and by what
+    its sum is off by (`err`), q_r by K u and the q's own errors, and p_j / p_r by
+    8 u of the distance d to the largest logit outside, where p_r is summed on its
+    own; where it is 1 less the entries' sum, p_r is at least q_r / 4 > 10^-4.6
+    and |log p_j| at most d + 11 + log V < d + 24."""
+    from pulsartecture_b200 import distill_topk
+
+    V = logits.shape[-1]
+    x = logits.double()
+    y = (x - x.amax(-1, keepdim=True)) / temperature
+    total = torch.logsumexp(y, -1, keepdim=True)
+    lp = y - total
+    lq = teacher.double() / temperature - lse.double()[:, None]
+    q = torch.exp(lq)
+    out = torch.ones_like(x, dtype=torch.bool).scatter_(-1, ids, False)
+    most_out = torch.where(out, x, -INF).amax(-1, keepdim=True)
+    below = torch.where(out, (x - most_out) / temperature, -INF)
+    sum_out = torch.logsumexp(below, -1, keepdim=True)
+    lpr = ((most_out - x.amax(-1, keepdim=True)) / temperature - total + sum_out)[:, 0]
+    qr = (1 - q.sum(-1)).clamp_min(0)
+    assert (qr > 1e-4).all()
+    given = torch.randn(len(x), generator=torch.Generator().manual_seed(9))
+    at = lp.gather(-1, ids)
+    want = (q * (lq - at)).sum(-1) + qr * (qr.log() - lpr)
+    leaf = logits.to(cuda).requires_grad_()
+    loss = distill_topk(leaf, ids.to(cuda), teacher.to(cuda), lse.to(cuda), temperature=temperature)
+    g, = torch.autograd.grad(loss, leaf, given.to(cuda))
+
+    p = torch.exp(lp)
+    err = _sum_error(V, lp, p)
+    size = teacher.double().abs().amax(-1) / temperature + lse.double().abs()
+    qerr = U * (8 + 4 * size + 2 * ids.shape[-1])
+    gap = 1 + torch.maximum(at.abs().amax(-1), lpr.abs())
+    _within(loss, want, (qerr * gap + 2 * err + 8 * U * gap) * 2, "loss")
+    c = (given.double() / temperature)[:, None]
+    ratio = torch.exp(below - sum_out)
+    one, two = p * (q.sum(-1) + qr)[:, None], qr[:, None] * ratio
+    value = c * torch.where(out, one - two, one - torch.zeros_like(p).scatter_add_(-1, ids, q))
+    d = torch.where(ratio > 0, -below, 0.0)
+    size_p = torch.where(p > 0, lp.abs(), 0.0)
+    most = one * (err[:, None] + 8 * U * (size_p + 24)) + two * (err[:, None] + U * (V / 128 + 40) + 8 * U * (d + 24))
+    most = most + qerr[:, None] * (p + ratio)
+    most.scatter_add_(-1, ids, (qerr[:, None] + 8 * U) * q)
+    # results and terms below 2^-126 flush to 0
+    _within(g, value, c.abs() * (most + 2.0 ** -125) + 4 * U * value.abs(), "dlogits")
+    return loss
+
+
+@pytest.mark.parametrize("rows,V", [(3, 40001), (200, 1000)])
+@pytest.mark.parametrize("scale", [1.0, 8.0, 20.0, 25.0, 40.0, 100.0, 1000.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_next_to_nothing_outside(cuda, rows, V, scale, dtype):
+    """The model's mass outside of the entries from its ordinary size down to
+    far below the smallest fp32 number: a finite loss, and a gradient there
+    that goes by what the teacher leaves."""
+    ids, top, lse, full = _teacher((rows,), V, 40, 5, 1.0)
+    assert torch.isfinite(_check_rest(cuda, (full * scale).to(dtype), ids, top, lse, 1.0)).all()
+
+
+@pytest.mark.parametrize("offset", [2e6, -3e6])
+def test_distill_next_to_nothing_outside_far_from_zero(cuda, offset):
+    for rows, V in ((3, 40001), (200, 1000)):
+        ids, top, lse, full = _teacher((rows,), V, 40, 5, 1.0)
+        _check_rest(cuda, full * 40 + offset, ids, top, lse, 1.0)
+
+
+def test_distill_some_of_the_rest_masked(cuda):
+    """Outside logits of -inf beside others far below the entries; then all of
+    them masked, by the type's lowest value and by -inf."""
+    from pulsartecture_b200 import distill_topk
+
+    V = 5003
+    ids, top, lse, full = _teacher((4,), V, 40, 5, 1.0)
+    logits = full * 40
+    out = torch.ones(4, V, dtype=torch.bool).scatter_(-1, ids, False)
+    logits[out & (torch.arange(V) % 3 > 0)] = -INF
+    _check_rest(cuda, logits, ids, top, lse, 1.0)
+    for dtype in TYPES:
+        for mask in (torch.finfo(dtype).min, -INF):
+            masked = logits.to(dtype)
+            masked[out] = mask
+            leaf = masked.to(cuda).requires_grad_()
+            loss = distill_topk(leaf, ids.to(cuda), top.to(cuda), lse.to(cuda))
+            g, = torch.autograd.grad(loss.sum(), leaf)
+            assert (loss == INF).all() and torch.isfinite(g).all() and not g.cpu()[out].any()
+
+
+@pytest.mark.parametrize("V,K", [(33, 7), (1000, 64), (4099, 200), (32000, 50), (50257, 17)])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("temperature", [1.0, 2.0])
+def test_distill_rest_gradient(cuda, V, K, dtype, temperature):
+    """The gradient of every logit outside of the entries by its own size."""
+    ids, top, lse, full = _teacher((6,), V, K, V + K, temperature)
+    logits = (full * 0.7 + torch.randn(6, V, generator=torch.Generator().manual_seed(K))).to(dtype)
+    _check_rest(cuda, logits, ids, top, lse, temperature)
