@@ -41,6 +41,7 @@ constexpr int kUnroll = 4;      // 16-byte loads of a thread in flight
 constexpr int kMaxCluster = 8;  // the largest portable cluster
 constexpr int kMaxTop = 32;     // as fakla_token_logprobs takes; also the lanes of a warp
 constexpr int kMaxEntries = 256;  // as fakla_distill_topk takes
+constexpr int kMaxVocab = 1 << 20;  // as all of them take
 constexpr int kCandidates = 512;
 constexpr int kOneWarp = 16;
 constexpr float kInf = __builtin_huge_valf();
@@ -771,26 +772,39 @@ struct Entries {
   }
 };
 
-// The teacher's entries of a row as a set: a table of ids, at most half full.
+// The teacher's entries of a row as a set: a table of ids, at most half full,
+// each with the first entry that names it. Which of several that is does not
+// depend on which came first to the table.
 constexpr int kSlots = 2 * kMaxEntries;
 struct EntrySet {
-  int slot[kSlots];  // -1: free
+  static constexpr uint32_t kFree = ~0u;
+  uint32_t slot[kSlots];  // id * kMaxEntries + entry
   __device__ __forceinline__ void clear() {
-    for (int i = threadIdx.x; i < kSlots; i += kThreads) slot[i] = -1;
+    for (int i = threadIdx.x; i < kSlots; i += kThreads) slot[i] = kFree;
   }
-  static __device__ __forceinline__ int place(int id) { return (int)((uint32_t)id * 2654435769u >> 23); }
-  // true for one of those that put the same id in
-  __device__ __forceinline__ bool put(int id) {
-    for (int h = place(id);; h = (h + 1) % kSlots) {
-      const int was = atomicCAS(&slot[h], -1, id);
-      if (was < 0 || was == id) return was < 0;
+  static __device__ __forceinline__ uint32_t place(uint32_t id) { return id * 2654435769u >> 23; }
+  // false where another entry of this id was in already
+  __device__ __forceinline__ bool put(uint32_t id, uint32_t entry) {
+    const uint32_t own = id * kMaxEntries + entry;
+    for (uint32_t h = place(id);; h = (h + 1) % kSlots) {
+      const uint32_t was = atomicCAS(&slot[h], kFree, own);
+      if (was == kFree) return true;
+      if (was / kMaxEntries != id) continue;
+      atomicMin(&slot[h], own);
+      return false;
     }
   }
-  __device__ __forceinline__ bool holds(int id) const {
-    for (int h = place(id);; h = (h + 1) % kSlots)
-      if (slot[h] < 0 || slot[h] == id) return slot[h] == id;
+  // the slot of id, or a free one
+  __device__ __forceinline__ uint32_t find(uint32_t id) const {
+    for (uint32_t h = place(id);; h = (h + 1) % kSlots) {
+      const uint32_t in = slot[h];
+      if (in == kFree || in / kMaxEntries == id) return in;
+    }
   }
+  __device__ __forceinline__ bool holds(int id) const { return find(id) != kFree; }
+  __device__ __forceinline__ bool is_first(int id, int entry) const { return find(id) % kMaxEntries == entry; }
 };
+static_assert((uint64_t)kMaxVocab * kMaxEntries < EntrySet::kFree, "a slot holds an id and an entry");
 static_assert(kSlots == 1 << (32 - 23), "place() gives a slot");
 
 // Both sums over the block, in every thread; once per N in a kernel.
@@ -921,7 +935,7 @@ __global__ void __launch_bounds__(kThreads, 12) distill_kernel(LogitsArgs p, int
   Running<T, false> run(scale_of(p));
   Entries entries;
   float given[kPerThread];  // the model's logits there
-  bool fresh[kPerThread];   // counted in P
+  bool fresh[kPerThread];   // the first of its id: counted in P
   Teacher t;
   auto first = [&] {
     if (rank != 0) return;
@@ -933,13 +947,15 @@ __global__ void __launch_bounds__(kThreads, 12) distill_kernel(LogitsArgs p, int
     bool twice = false;
 #pragma unroll
     for (int i = 0; i < kPerThread; ++i) {
-      fresh[i] = false;
       if (entries.id[i] < 0) continue;
-      fresh[i] = set.put(entries.id[i]);
-      twice |= !fresh[i];
+      twice |= !set.put(entries.id[i], threadIdx.x + i * kThreads);
     }
     __syncwarp();  // threads that looked further are waited for here, not all along the row
-    t = teacher_stats(p, entries, twice);
+    t = teacher_stats(p, entries, twice);  // (has a barrier: the table is complete)
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i)
+      fresh[i] = entries.id[i] >= 0 && (!t.twice || set.is_first(entries.id[i], threadIdx.x + i * kThreads));
+    __syncwarp();
   };
   each_vectors(row, v0, v1, first, [&](const uint4* raw, int v) {
     float top = -kInf;

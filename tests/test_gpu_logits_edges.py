@@ -234,3 +234,29 @@ def test_distill_rest_gradient(cuda, V, K, dtype, temperature):
     ids, top, lse, full = _teacher((6,), V, K, V + K, temperature)
     logits = (full * 0.7 + torch.randn(6, V, generator=torch.Generator().manual_seed(K))).to(dtype)
     _check_rest(cuda, logits, ids, top, lse, temperature)
+
+
+@pytest.mark.parametrize("rows,V", [(6, 40000), (3000, 2000)])  # (rows start alike on 16 bytes)
+def test_distill_repeated_entries_are_the_same_bits(cuda, rows, V):
+    """Rows that are all alike, with ids named by several warps' threads, most
+    of the model's mass at them and a small divergence: one loss and one
+    gradient, on every row and every run."""
+    from pulsartecture_b200 import distill_topk
+
+    g = torch.Generator().manual_seed(1)
+    K = 256
+    full = torch.randn(V, generator=g)
+    ids = torch.randint(0, 90, (K,), generator=g) * (V // 91)
+    full[ids] += 8.0
+    logits = full.expand(rows, V).contiguous().to(cuda).requires_grad_()
+    top = full[ids] + 0.2 * torch.randn(K, generator=g)
+    lse = torch.logsumexp(top, 0) + 0.2
+    args = [ids.expand(rows, K).to(cuda), top.expand(rows, K).to(cuda), lse.expand(rows).to(cuda)]
+    first = None
+    for _ in range(20):
+        loss = distill_topk(logits, *args)
+        grad, = torch.autograd.grad(loss.sum(), logits)
+        if first is None:
+            first = loss[0].item(), grad[0].clone()
+        assert (loss == first[0]).all()
+        assert (grad == first[1]).all()
