@@ -23,6 +23,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "fakla_common.cuh"
@@ -1179,10 +1180,11 @@ __global__ void __launch_bounds__(kThreads) distill_backward_kernel(LogitsArgs p
 // alternatives took 34, 34 and 41 us, 257 x 50257 bf16 distillation (forward and
 // backward) 21, 22 and 21.
 constexpr int kBlocks = 4;
+constexpr int kClusterBytes = 48 << 10;
 int cluster_size(int64_t rows, int64_t vectors, int bytes) {
   int c = 1;
   while (c < kMaxCluster && ((rows * c < kBlocks * fakla_sm_count() && vectors / (2 * c) >= kThreads) ||
-                             vectors / c * bytes > (48 << 10)))
+                             vectors / c * bytes > kClusterBytes))
     c *= 2;
   return c;
 }
@@ -1193,7 +1195,10 @@ cudaError_t launch_rows(K kernel, const LogitsArgs& p, int per_vector, int bytes
   const int c = cluster_size(p.batch * p.rows, vectors, bytes);
   const size_t smem = ((size_t)((vectors + c - 1) / c + 1) * bytes + 15) / 16 * 16;
   if (smem > (32 << 10)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // The limit belongs to the kernel, which other threads launch at the same
+    // time: it is the most that any call asks for, never this call's size.
+    const int most = std::max(kMaxVocab / per_vector / kMaxCluster * bytes, kClusterBytes) + 64;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return e;
   }
   return launch_chained(kernel, dim3((unsigned)(p.batch * p.rows * c)), dim3(kThreads), smem, stream, (unsigned)c, p, c);

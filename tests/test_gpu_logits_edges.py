@@ -260,3 +260,41 @@ def test_distill_repeated_entries_are_the_same_bits(cuda, rows, V):
             first = loss[0].item(), grad[0].clone()
         assert (loss == first[0]).all()
         assert (grad == first[1]).all()
+
+
+def test_alternatives_from_two_threads(cuda):
+    """Vocabularies that ask for different amounts of shared memory, scored by
+    two threads at once: each call is as valid as alone."""
+    from pulsartecture_b200 import _lib, token_logprobs
+
+    errors, found = [], {}
+    start = threading.Barrier(2)
+
+    def work(V):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                logits = torch.zeros(1, V, device=cuda)
+                logits[:, 9] = 1.0
+                targets = torch.zeros(1, dtype=torch.int64, device=cuda)
+                r = token_logprobs(logits, targets, top_k=2)
+                stream.synchronize()
+                call = _lib.lib().fakla_token_logprobs
+                args = [t.data_ptr() for t in (logits, targets, r.logprobs, r.entropy, r.top_logprobs, r.top_ids)]
+                args += [None, 1, 1, V, V, V, 2, 1.0, -100, _lib.FAKLA_F32, stream.cuda_stream]
+                start.wait(60)
+                for _ in range(20000):
+                    _lib.check(call(*args))
+                stream.synchronize()
+                found[V] = r.top_ids.tolist()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    sizes = (270000, 1000000)
+    threads = [threading.Thread(target=work, args=(V,)) for V in sizes]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(300)
+    assert not errors, errors[0]
+    assert all(found[V] == [[9, 0]] for V in sizes)
