@@ -747,11 +747,14 @@ int check_gated_scan(int64_t B, int64_t T, int64_t D, int act, int dtype) {
 }
 
 // Every pointer on a multiple of its element (null is).
-int check_elements(std::initializer_list<const void*> values, std::initializer_list<const void*> floats, int dtype) {
+int check_elements(std::initializer_list<const void*> values, std::initializer_list<const void*> floats, int dtype,
+                   std::initializer_list<const int64_t*> ids = {}) {
   for (const void* p : values)
     if ((uintptr_t)p % esize(dtype)) return fakla_set_error(FAKLA_ERR_ALIGNMENT, "a tensor does not start on an element");
   for (const void* p : floats)
     if ((uintptr_t)p % sizeof(float)) return fakla_set_error(FAKLA_ERR_ALIGNMENT, "an fp32 tensor does not start on an element");
+  for (const int64_t* p : ids)
+    if ((uintptr_t)p % sizeof(int64_t)) return fakla_set_error(FAKLA_ERR_ALIGNMENT, "an int64 tensor does not start on an element");
   return FAKLA_OK;
 }
 
@@ -859,7 +862,6 @@ int check_logits(const void* logits, int64_t batch, int64_t rows, int64_t vocab,
   int rc = check_dtype(dtype);
   if (rc) return rc;
   if (!logits) return fakla_set_error(FAKLA_ERR_INVALID_ARG, "logits must be non-NULL");
-  if ((rc = check_elements({logits}, {}, dtype))) return rc;
   if (batch < 1 || rows < 1 || vocab < 1)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG, "sizes must be positive (batch=%lld rows=%lld vocab=%lld)",
                            (long long)batch, (long long)rows, (long long)vocab);
@@ -903,6 +905,7 @@ extern "C" int fakla_token_logprobs(const void* logits, const int64_t* targets, 
   if (!targets || !logprobs || !entropy || (top_k > 0 && (!top_logprobs || !top_ids)))
     return fakla_set_error(FAKLA_ERR_INVALID_ARG,
                            "targets, logprobs, entropy and (with top_k) top_logprobs, top_ids must be non-NULL");
+  if ((rc = check_elements({logits}, {logprobs, entropy, top_logprobs, stats}, dtype, {targets, top_ids}))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   p.batch_stride = batch_stride;
@@ -934,7 +937,8 @@ extern "C" int fakla_token_logprobs_backward(const void* logits, const int64_t* 
   if (!targets || !stats || !entropy || !dlogits || (dtop_logprobs && (!top_ids || top_k == 0)))
     return fakla_set_error(FAKLA_ERR_INVALID_ARG,
                            "targets, stats, entropy, dlogits and (with dtop_logprobs) top_ids must be non-NULL");
-  if ((rc = check_elements({dlogits}, {}, dtype))) return rc;
+  if ((rc = check_elements({logits, dlogits}, {stats, entropy, dlogprobs, dentropy, dtop_logprobs}, dtype, {targets, top_ids})))
+    return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   p.batch_stride = batch_stride;
@@ -964,6 +968,7 @@ extern "C" int fakla_distill_topk(const void* logits, const int64_t* teacher_ids
   if (rc) return rc;
   if (!teacher_ids || !teacher_logits || !loss)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG, "teacher_ids, teacher_logits and loss must be non-NULL");
+  if ((rc = check_elements({logits}, {teacher_logits, teacher_lse, loss, stats}, dtype, {teacher_ids}))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   p.batch_stride = batch_stride;
@@ -992,7 +997,7 @@ extern "C" int fakla_distill_topk_backward(const void* logits, const int64_t* te
   if (!teacher_ids || !teacher_logits || !stats || !dloss || !dlogits)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG,
                            "teacher_ids, teacher_logits, stats, dloss and dlogits must be non-NULL");
-  if ((rc = check_elements({dlogits}, {}, dtype))) return rc;
+  if ((rc = check_elements({logits, dlogits}, {teacher_logits, teacher_lse, stats, dloss}, dtype, {teacher_ids}))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   p.batch_stride = batch_stride;

@@ -156,3 +156,25 @@ def test_oracles_agree_with_autograd():
         want, = torch.autograd.grad(total, z, retain_graph=True)
         got = logits_oracle.distill(z.detach(), ids, teacher, lse, 0.7, dlp)
         assert torch.allclose(got["dlogits"], want, rtol=1e-10, atol=1e-10)
+
+
+def test_logits_pointers_off_their_elements():
+    """Every pointer of the logits entry points is refused where it is not on a
+    multiple of its element: a kernel could not read or write there."""
+    _no_gpu()
+    L = _lib.lib()
+    calls = {
+        # pointers, in order: T = logits' type (fp32 here), f = fp32, i = int64
+        "fakla_token_logprobs": ("Tifffif", [1, 1, 100, 100, 100, 4, 1.0, -100, 0]),
+        "fakla_token_logprobs_backward": ("TiffifffT", [1, 1, 100, 100, 100, 4, 1.0, -100, 0]),
+        "fakla_distill_topk": ("Tiffff", [1, 1, 100, 100, 100, 4, 1.0, 0]),
+        "fakla_distill_topk_backward": ("TiffffT", [1, 1, 100, 100, 100, 4, 1.0, 0]),
+    }
+    for name, (kinds, rest) in calls.items():
+        fn = getattr(L, name)
+        assert fn(*[P] * len(kinds), *rest, None) in (4, 7), name
+        for n, kind in enumerate(kinds):
+            for off in (18, 20):
+                args = [P] * len(kinds)
+                args[n] = ctypes.c_void_p(off)
+                assert (fn(*args, *rest, None) == 3) == (off % (8 if kind == "i" else 4) != 0), (name, n, off)
