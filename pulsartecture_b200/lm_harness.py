@@ -159,6 +159,8 @@ class FaklaLM(nn.Module):
 
     def distill_loss(self, ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
                      teacher_lse: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
-        """Mean over ids (B, T) of the KL divergence from a teacher's largest
-        logits, teacher_ids and teacher_logits (B, T, K)."""
-        return distill_topk(self(ids), teacher_ids, teacher_logits, teacher_lse, temperature=temperature).mean()
+        """Mean KL divergence from a teacher's largest logits, teacher_ids and
+        teacher_logits (B, T, K), over the positions of ids (B, T) that have an
+        entry (an id that is not -1)."""
+        losses = distill_topk(self(ids), teacher_ids, teacher_logits, teacher_lse, temperature=temperature)
+        return losses.sum() / (teacher_ids != -1).any(-1).sum().clamp_min(1)
