@@ -140,10 +140,15 @@ class FaklaLM(nn.Module):
         return self.head(self.ln_f(x))
 
     @torch.no_grad()
-    def score(self, ids: torch.Tensor, top_k: int = 0, temperature: float = 1.0) -> TokenLogprobs:
+    def score(self, ids: torch.Tensor, top_k: int = 0, temperature: float = 1.0,
+              ignore_index: int = -100) -> TokenLogprobs:
         """What the model gave the tokens ids[:, 1:] in their places: (B, T - 1)
-        log probabilities and entropies, with the top_k alternatives of each."""
-        return token_logprobs(self(ids)[:, :-1], ids[:, 1:], top_k=top_k, temperature=temperature)
+        log probabilities and entropies, with the top_k alternatives of each.
+        Padding (ids of ignore_index) is embedded as token 0 and has log
+        probability 0; entropies and alternatives are given there too."""
+        logits = self(ids.masked_fill(ids == ignore_index, 0))
+        return token_logprobs(logits[:, :-1], ids[:, 1:], top_k=top_k, temperature=temperature,
+                              ignore_index=ignore_index)
 
     def loss(self, ids: torch.Tensor, entropy_weight: float = 0.0, ignore_index: int = -100) -> torch.Tensor:
         """Mean next-token cross entropy of ids (B, T), less entropy_weight times
@@ -158,9 +163,14 @@ class FaklaLM(nn.Module):
         return -total / counted.sum().clamp_min(1)
 
     def distill_loss(self, ids: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
-                     teacher_lse: Optional[torch.Tensor] = None, temperature: float = 1.0) -> torch.Tensor:
+                     teacher_lse: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                     ignore_index: int = -100) -> torch.Tensor:
         """Mean KL divergence from a teacher's largest logits, teacher_ids and
         teacher_logits (B, T, K), over the positions of ids (B, T) that have an
-        entry (an id that is not -1)."""
-        losses = distill_topk(self(ids), teacher_ids, teacher_logits, teacher_lse, temperature=temperature)
+        entry (an id that is not -1). Padding (ids of ignore_index) is embedded
+        as token 0 and left out."""
+        padding = ids == ignore_index
+        teacher_ids = teacher_ids.masked_fill(padding[..., None], -1)
+        losses = distill_topk(self(ids.masked_fill(padding, 0)), teacher_ids, teacher_logits, teacher_lse,
+                              temperature=temperature)
         return losses.sum() / (teacher_ids != -1).any(-1).sum().clamp_min(1)

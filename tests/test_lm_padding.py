@@ -52,3 +52,24 @@ def test_positions_without_a_teacher_do_not_count(model, rest):
     got = model.distill_loss(ids, t_ids, top, lse)
     assert abs(float(got - per.sum() / (12 + 7))) < 1e-12
     assert float(model.distill_loss(ids, torch.full_like(t_ids, -1), top, lse)) == 0.0
+
+
+def test_padded_ids_are_not_embedded(model):
+    """Padding (ignore_index) in score and distill_loss, as in loss."""
+    ids, t_ids, top, lse = _batch()
+    padded = ids.clone()
+    padded[1, 7:] = -100
+    padded[2, :] = -100
+    r, w = model.score(padded, top_k=2), model.score(ids, top_k=2)
+    assert r.logprobs.shape == (3, 11) and r.top_ids.shape == (3, 11, 2)
+    assert torch.equal(r.logprobs[0], w.logprobs[0]) and torch.equal(r.logprobs[1, :6], w.logprobs[1, :6])
+    assert not r.logprobs[1, 6:].any() and not r.logprobs[2].any()
+    got = model.distill_loss(padded, t_ids, top, lse)
+    per = lm_harness.distill_topk(model(ids), t_ids, top, lse)
+    assert abs(float(got - (per[0].sum() + per[1, :7].sum()) / 19)) < 1e-12
+    # another mark, which is a token of the vocabulary
+    marked = ids.clone()
+    marked[0, 9:] = 5
+    a = model.score(marked, ignore_index=5)
+    assert not a.logprobs[0, 8:].any()
+    assert float(model.distill_loss(torch.full_like(ids, -7), t_ids, top, ignore_index=-7)) == 0.0
