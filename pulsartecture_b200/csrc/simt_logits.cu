@@ -920,10 +920,12 @@ __device__ __forceinline__ Outside sum_outside(const Row<T>& row, const EntrySet
 // that sum in the pass, by a byte of marks per vector, took 8 us of the 59 of
 // 4096 x 32000 bf16 with 64 entries.) The ratio q_r / p_r is 1 + (P - Q) / p_r, whose
 // difference keeps its digits where the entries hold little: the quotient is
-// off by up to 2 10^-5 of such a loss, this by 10^-6. Twelve blocks on an SM (40
-// registers a thread) take 49 us for 4096 x 32000 bf16, nine of 56 registers 51.
+// off by up to 2 10^-5 of such a loss, this by 10^-6. Where every
+// row is walked (K = 16), 4096 x 32000 bf16 takes 270 us instead of 50. Twelve
+// blocks on an SM (40 registers a thread, 8 to 16 bytes of them spilled) or
+// nine (56 registers): bf16 50 and 53 us, 2048 x 32000 fp32 51 and 47.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 12) distill_kernel(LogitsArgs p, int C) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 12 : 9) distill_kernel(LogitsArgs p, int C) {
   __shared__ EntrySet set;
   __shared__ Sums peers[kMaxCluster];
   griddep_wait();
