@@ -53,7 +53,7 @@ typedef enum fakla_status {
   FAKLA_OK = 0,
   FAKLA_ERR_INVALID_ARG = 1, /* null pointer, non-positive size, bad flag */
   FAKLA_ERR_UNSUPPORTED = 2, /* well-formed but outside the implemented set */
-  FAKLA_ERR_ALIGNMENT = 3,   /* a pointer lacks the 16-byte alignment needed */
+  FAKLA_ERR_ALIGNMENT = 3,   /* a pointer lacks the alignment needed */
   FAKLA_ERR_CUDA = 4,        /* CUDA runtime error while launching */
   FAKLA_ERR_TIMEOUT = 5,     /* a bounded device-side wait expired */
   FAKLA_ERR_WORKSPACE = 6,   /* workspace missing or smaller than required */

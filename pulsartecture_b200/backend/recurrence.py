@@ -105,11 +105,12 @@ def gated_scan(x: torch.Tensor, gate: torch.Tensor, state: Optional[torch.Tensor
     x, gate: (B, T, D), float32 or bfloat16; column blocks of a wider tensor
     (``proj.chunk(2, -1)``) and expanded batch or time dimensions are read in
     place. gate_act: "sigmoid" (a = sigmoid(gate)) or "identity" (a = gate, a
-    decay factor: products of up to 64 consecutive ones have to fit float32).
-    mix: b = (1 - a) x, otherwise b = x. state: (B, D) float32, h before the
-    first token, or None for zero; it is not modified. h is carried in float32
-    and rounded to the input dtype in the output; the final state (B, D) is
-    float32. Differentiable in x, gate and state, through both results.
+    decay factor: products of up to 64 consecutive ones have to fit float32;
+    bfloat16 has none between 1 - 2^-8 and 1, so slower decays need float32 x
+    and gate). mix: b = (1 - a) x, otherwise b = x. state: (B, D) float32, h
+    before the first token, or None for zero; it is not modified. h is carried
+    in float32 and rounded to the input dtype in the output; the final state
+    (B, D) is float32. Differentiable in x, gate and state, through both results.
 
     A gate of -inf ("sigmoid") or 0 ("identity") forgets the state, so packed
     documents are separated by setting it at their first tokens.
