@@ -401,7 +401,7 @@ int fakla_decode_noalloc(const void* q, const void* k, const void* v,
  *   out       : (B, T, D) dense, written: h_t rounded to dtype
  *   state_in  : (B, D) fp32, h before the first token, or NULL for zero
  *   state_out : (B, D) fp32, written with h after the last token, or NULL;
- *               may be state_in
+ *               may be state_in, and otherwise does not overlap it
  *   saved     : fakla_gated_scan_saved_bytes() that the backward reads, or NULL
  * h is carried in fp32. A gate of -inf (sigmoid) or 0 (identity) starts a new
  * sequence at its token. Identity gates are decay factors: products of up to

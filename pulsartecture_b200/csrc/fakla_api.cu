@@ -758,6 +758,15 @@ int check_elements(std::initializer_list<const void*> values, std::initializer_l
   return FAKLA_OK;
 }
 
+// The (B, D) state is written over the one that is read, or apart from it.
+int check_states(const float* in, const float* out, int64_t B, int64_t D) {
+  if (!in || !out || in == out) return FAKLA_OK;
+  const uintptr_t a = (uintptr_t)in, b = (uintptr_t)out, bytes = (uintptr_t)B * (uintptr_t)D * sizeof(float);
+  if ((a < b ? b - a : a - b) < bytes)
+    return fakla_set_error(FAKLA_ERR_INVALID_ARG, "state_out overlaps state_in in part");
+  return FAKLA_OK;
+}
+
 // The strides of a dimension of one row do not matter: 0 keeps every alignment.
 void set_inputs(fakla::GatedScanArgs* p, const void* x, const void* gate, int64_t B, int64_t T, int64_t D,
                 int64_t x_batch, int64_t x_time, int64_t gate_batch, int64_t gate_time, int act, int mix) {
@@ -788,6 +797,7 @@ extern "C" int fakla_gated_scan(const void* x, const void* gate, void* out, cons
   if (rc) return rc;
   if (!x || !gate || !out) return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate and out must be non-NULL");
   if ((rc = check_elements({x, gate, out}, {state_in, state_out, saved}, dtype))) return rc;
+  if ((rc = check_states(state_in, state_out, B, D))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};
@@ -836,6 +846,7 @@ extern "C" int fakla_gated_scan_step(const void* x, const void* gate, void* out,
   if (!x || !gate || !out || !state_in || !state_out)
     return fakla_set_error(FAKLA_ERR_INVALID_ARG, "x, gate, out, state_in and state_out must be non-NULL");
   if ((rc = check_elements({x, gate, out}, {state_in, state_out}, dtype))) return rc;
+  if ((rc = check_states(state_in, state_out, N, D))) return rc;
   DeviceInfo* d = nullptr;
   if ((rc = require_device(&d))) return rc;
   fakla::GatedScanArgs p = {};

@@ -178,3 +178,17 @@ def test_logits_pointers_off_their_elements():
                 args = [P] * len(kinds)
                 args[n] = ctypes.c_void_p(off)
                 assert (fn(*args, *rest, None) == 3) == (off % (8 if kind == "i" else 4) != 0), (name, n, off)
+
+
+def test_states_that_overlap_in_part():
+    """state_out is state_in or apart from it: blocks read the one while others
+    write the other."""
+    _no_gpu()
+    L = _lib.lib()
+    N, D = 4, 8
+    size = N * D * 4
+    for off, refused in ((0, False), (4, True), (size - 4, True), (-4, True), (4 - size, True), (size, False), (-size, False)):
+        a, b = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + off)
+        for rc in (L.fakla_gated_scan_step(P, P, P, a, b, N, D, D, D, 5, 1, 1, None),
+                   L.fakla_gated_scan(P, P, P, a, b, None, N, 3, D, 3 * D, D, 3 * D, D, 5, 1, 1, None)):
+            assert (rc == 1 and b"overlap" in L.fakla_last_error()) if refused else rc in (4, 7), off
